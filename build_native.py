@@ -21,6 +21,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 NATIVE = os.path.join(ROOT, "native")
@@ -171,19 +172,27 @@ def build_bw_sweep():
 
 
 def build_fused_ops():
-    """Fused normalization kernels (gfx950)."""
+    """Fused decode kernels, paged KV cache and its attention (gfx950)."""
 
-    srcs = [os.path.join(NATIVE, "ops", "fused_ops.hip"),
-            os.path.join(NATIVE, "ops", "skinny_gemm.hip")]
-    srcs = [s0 for s0 in srcs if os.path.exists(s0)]
-    if not srcs:
-        return None
+    srcs = [os.path.join(NATIVE, "ops", f) for f in (
+        "paged_attention.hip", "paged_cache.hip", "fused_ops.hip",
+        "skinny_gemm.hip")]
     os.makedirs(OUT, exist_ok=True)
     target = os.path.join(OUT, "libtfops.so")
-    if not _newer(target, srcs):
+    if not _newer(target, srcs + [os.path.join(NATIVE, "ops",
+                                               "paged_common.h")]):
         return target
-    _run([HIPCC] + HIPFLAGS + ["-O3", "-std=c++17", "-fPIC",
-          "-shared"] + srcs + ["-o", target])
+    # one compiler for each source, side by side
+    objs = [os.path.join(OUT, os.path.basename(s0)[:-4] + ".o")
+            for s0 in srcs]
+    with ThreadPoolExecutor(len(srcs)) as pool:
+        list(pool.map(lambda so: _run(
+            [HIPCC] + HIPFLAGS + ["-O3", "-std=c++17", "-fPIC", "-c", so[0],
+                                  "-o", so[1]]), zip(srcs, objs)))
+    _run([HIPCC, "--offload-arch=gfx950", "-shared"] + objs
+         + ["-o", target])
+    for o in objs:
+        os.remove(o)
     return target
 
 

@@ -1,0 +1,1057 @@
+// Attention of new tokens over a paged KV cache on gfx950.
+//
+//   out[i,h] = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i.k_j - m_i)
+//
+// for the packed rows i of a ragged batch, over the pages of each sequence;
+// causal: row t of a chunk of n new tokens sees the first len - n + t + 1 of
+// the sequence's len keys. One pass over the keys with the running maximum
+// and sum. Statistics, scores and the sum over p v are 32 bits; p is rounded
+// to the rows' 16-bit type for the matrix product (half a step of 2^-8 or
+// 2^-11 each, independent over the keys), the result once more.
+//
+// Rows: the G = Hq / Hk query heads that share a kv head are rows of one
+// tile, row r = t * G + g, so that a key is fetched once for all of them.
+// Both kernels work on S^T = K Q^T and O^T = V^T P^T: a column of the
+// result is a query row, so a lane keeps one row's statistics, and what S^T
+// leaves in a lane's registers is, with the keys of a step permuted in V
+// likewise, what P^T takes: p never leaves the registers.
+//
+//   few:  tiles of 16 or 32 rows, 4 waves that each take every fourth tile
+//         of 32 keys by themselves and are joined at the end. K goes from
+//         memory to registers, V through the wave's own LDS and comes back
+//         by transposing reads. Bound by HBM.
+//   many: tiles of 128 rows, 4 waves of 32 rows over shared tiles of 64
+//         keys in LDS, two of them in turn. Bound by the matrix and vector
+//         pipes.
+//
+// Both split the keys over gridDim.y where tiles are few; `join` adds the
+// parts. How many splits work is settled on the device, by the sequence's
+// own length.
+//
+// Keys that a row does not see have p = 0 by selection; V rows past the end
+// enter as 0; where rows of a tile see different keys and V holds NaN or
+// infinities, the tile takes a path that keeps those from rows that do not
+// see them. A page number outside of the pool makes the scores of its keys
+// NaN; a length that the table cannot hold makes its rows NaN. Nothing
+// outside of the tensors is read.
+
+#include "paged_common.h"
+
+namespace {
+
+using namespace paged;
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  const int* q_starts;
+  const int* kv_lens;
+  const int* table;
+  void* out;
+  float* parts;  // [tile * Hk + h][split][row]: D sums, then maximum and sum
+  long long q_row, q_head, table_row;
+  int cols;  // of the table
+  int T, B, Hq, Hk, G, pages, page_log2;
+  float scale;  // times log2(e): exponentials are of base 2
+  int causal, splits;
+  int which;  // 0: all sequences, 1: those of at most 32 rows, 2: the others
+};
+
+constexpr int FEW_ROWS = 32;
+
+// ---- what is where ----------------------------------------------------
+
+struct Span {
+  int seq = -1;
+  int row0, rows;  // the tile's first row, the sequence's rows
+  int q0, n, len;  // first packed token, new tokens, keys
+  bool broken;     // a length that the table cannot hold
+};
+
+// Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
+// leaves each at least its own number, needs no sum over the sequences
+// before it, and the last such start at or below `tile` is its sequence.
+__device__ inline Span find(const Args& a, int tile, int BM) {
+  Span s;
+  int seq;
+  if (a.which == 1) {
+    seq = tile;
+  } else {
+    const int lane = threadIdx.x & 63;
+    seq = -1;
+    for (int base = 0; base < a.B; base += 64) {
+      int i = base + lane;
+      bool at = false;
+      if (i < a.B) {
+        int start = min(max(a.q_starts[i], 0), a.T);
+        at = start * a.G / BM + i <= tile;
+      }
+      int c = __popcll(__ballot(at));
+      seq += c;
+      if (c < 64) break;
+    }
+  }
+  if (seq < 0 || seq >= a.B) return s;
+  int q0 = min(max(a.q_starts[seq], 0), a.T);
+  int q1 = min(max(a.q_starts[seq + 1], 0), a.T);
+  s.n = q1 - q0;
+  s.rows = s.n * a.G;
+  s.q0 = q0;
+  s.row0 = a.which == 1 ? 0 : (tile - (q0 * a.G / BM + seq)) * BM;
+  if (s.row0 >= s.rows || s.row0 < 0) return s;
+  if (a.which == 1 && s.rows > FEW_ROWS) return s;
+  if (a.which == 2 && s.rows <= FEW_ROWS) return s;
+  s.len = a.kv_lens[seq];
+  const long long room = (long long)a.cols << a.page_log2;
+  s.broken = s.len < 0 || s.len > room;
+  if (s.broken) s.len = 0;
+  s.seq = seq;
+  return s;
+}
+
+// how many of the sequence's keys row r sees
+__device__ inline int seen_by(const Args& a, const Span& s, int r) {
+  if (r >= s.rows) return 0;
+  if (!a.causal) return s.len;
+  return min(max(s.len - s.n + r / a.G + 1, 0), s.len);
+}
+
+// tiles of keys: what this split takes of `all`, and how many splits work
+struct Share {
+  int first, last, active;
+};
+
+__device__ inline Share share_of(int all, int splits, int split, int least) {
+  int each = max((all + splits - 1) / splits, least);
+  Share s;
+  s.active = max((all + each - 1) / each, 1);
+  s.first = min(split * each, all);
+  s.last = min(s.first + each, all);
+  return s;
+}
+
+// ---- small pieces ------------------------------------------------------
+
+__device__ inline float lane_xor16_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x),
+                                            __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float lane_xor32_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                            __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float lane_xor16_add(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x),
+                                            __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline float lane_xor32_add(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                            __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float minus_inf() { return __uint_as_float(0xff800000u); }
+__device__ inline float plus_inf() { return __uint_as_float(0x7f800000u); }
+// a maximum to subtract: nothing has been seen where it is -inf
+__device__ inline float base_of(float m) {
+  return m == minus_inf() ? 0.0f : m;
+}
+
+__device__ inline f4 mfma16(Bf16::V8 a, Bf16::V8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f4 mfma16(Fp16::V8 a, Fp16::V8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f16v mfma32(Bf16::V8 a, Bf16::V8 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f16v mfma32(Fp16::V8 a, Fp16::V8 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// 8 codes times their scale, rounded to 16 bits: exact, but for fp16 where
+// the value is not one of fp16's
+__device__ inline void widen(Oct<Bf16>& o, u2 codes, float scale) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[j], scale, false);
+    auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[j], scale, true);
+    o.h[4 * j] = lo[0];
+    o.h[4 * j + 1] = lo[1];
+    o.h[4 * j + 2] = hi[0];
+    o.h[4 * j + 3] = hi[1];
+  }
+}
+__device__ inline void widen(Oct<Fp16>& o, u2 codes, float scale) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale, false);
+    auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale, true);
+    o.h[4 * j] = lo[0];
+    o.h[4 * j + 1] = lo[1];
+    o.h[4 * j + 2] = hi[0];
+    o.h[4 * j + 3] = hi[1];
+  }
+}
+
+__device__ inline bool strange(const Oct<Bf16>& o) {
+  bool s = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    s |= (o.raw[j] & 0x7f80u) == 0x7f80u ||
+         (o.raw[j] & 0x7f800000u) == 0x7f800000u;
+  return s;
+}
+__device__ inline bool strange(const Oct<Fp16>& o) {
+  bool s = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    s |= (o.raw[j] & 0x7c00u) == 0x7c00u ||
+         (o.raw[j] & 0x7c000000u) == 0x7c000000u;
+  return s;
+}
+
+// V's values for the tiles that hold NaN or infinities: the finite ones
+// (kind 0), or 1 where a value is NaN, +inf, -inf (kinds 1, 2, 3)
+template <typename K>
+__device__ inline Oct<K> only(Oct<K> o, int kind) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float x = (float)o.h[j];
+    bool finite = fabsf(x) < plus_inf();
+    float y = kind == 0   ? (finite ? x : 0.0f)
+              : kind == 1 ? (x != x ? 1.0f : 0.0f)
+              : kind == 2 ? (x == plus_inf() ? 1.0f : 0.0f)
+                          : (x == minus_inf() ? 1.0f : 0.0f);
+    o.h[j] = (typename K::T)y;
+  }
+  return o;
+}
+__device__ inline float special(int kind) {
+  return kind == 1 ? nan_f32() : kind == 2 ? plus_inf() : minus_inf();
+}
+
+typedef __attribute__((address_space(3))) s4* lds_s4;
+
+// 4 keys by 16 values, transposed: a lane of 16 names 4 values of key
+// (lane >> 2), and gets the 4 keys of value (lane & 15)
+__device__ inline u2 transposed(const void* p) {
+  s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_s4)(const __attribute__((address_space(3))) void*)p);
+  return __builtin_bit_cast(u2, r);
+}
+
+__device__ inline void wave_fence() {
+  // LDS of one wave: its accesses are done in order, the compiler is told
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ---- few rows ------------------------------------------------------------
+
+// Where 16-byte piece c of a wave's V row lies: the 32-byte blocks that a
+// transposing read takes from 8 neighbouring rows fall on different banks.
+template <int D>
+__device__ inline int few_piece(int row, int c) {
+  if constexpr (D == 128) return c ^ ((row & 7) << 1);
+  if constexpr (D == 64) return c ^ (((row >> 1) & 3) << 1);
+  return c ^ (((row >> 2) & 1) << 1);
+}
+
+template <typename K, int D, bool Q8, int RT>
+__global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
+  typedef typename K::T T;
+  constexpr int BM = 16 * RT, BN = 32, WAVES = 4;
+  constexpr int NF = D / 32;              // steps of the product over D
+  constexpr int NT = D / 16;              // tiles of 16 values of O^T
+  constexpr int EB = Q8 ? 1 : 2;          // bytes of a cached value
+  constexpr int LPR = D * EB / 16;        // lanes for one V row
+  constexpr int VROWS = 64 / LPR;         // V rows of one load
+  constexpr int NV = BN / VROWS;          // loads for a tile of V
+  constexpr int KB = NF * 8 * EB >= 16 ? 16 : 8;  // bytes of a K load
+  constexpr int NK = NF * 8 * EB / KB;    // K loads of a lane for 16 keys
+  constexpr int JS = D + 4;               // a row of what the waves join
+
+  // V tiles while the keys pass, then the waves' sums
+  __shared__ __attribute__((aligned(16))) char
+      lds[WAVES * 16 * JS * 4 > WAVES * BN * D * 2 ? WAVES * 16 * JS * 4
+                                                   : WAVES * BN * D * 2];
+  __shared__ float stat[2][WAVES][16];
+
+  const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
+  const Span s = find(a, tile, BM);
+  if (s.seq < 0) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = lane & 15, grp = lane >> 4;
+
+  const int seen_min = seen_by(a, s, s.row0);
+  const int last_row = min(s.row0 + BM, s.rows) - 1;
+  const int seen_max = seen_by(a, s, last_row);
+  const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
+                              2 * WAVES);
+  if ((int)blockIdx.y >= mine.active) return;
+
+  // Q: a lane holds 8 values of row `col` for each step
+  Oct<K> q[RT][NF];
+  int seen[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = s.row0 + rt * 16 + col;
+    seen[rt] = seen_by(a, s, r);
+    const bool real = r < s.rows;
+    const int t = real ? r / a.G : 0, g = real ? r % a.G : 0;
+    const T* src = (const T*)a.q + (s.q0 + t) * a.q_row +
+                   (long long)(h * a.G + g) * a.q_head;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const int d0 = KB == 16 && Q8 ? 64 * (f >> 1) + grp * 16 + (f & 1) * 8
+                                    : 32 * f + grp * 8;
+      q[rt][f].raw = real ? *reinterpret_cast<const u4*>(src + d0)
+                          : u4{0, 0, 0, 0};
+    }
+  }
+
+  const int* pages = a.table + s.seq * a.table_row;
+  const uint8_t* kc = (const uint8_t*)a.k;
+  const uint8_t* vc = (const uint8_t*)a.v;
+  const int in_page = (1 << a.page_log2) - 1;
+
+  // pages of the two halves of tile kt; keys past the last are not looked up
+  auto page_of = [&](int key) {
+    int p = key < seen_max ? pages[key >> a.page_log2] : 0;
+    return p;
+  };
+
+  u4 kr[2][NK], vr[NV];
+  uint32_t ksr[2], vsr[NV];
+  int id[2], nid[2];  // of the tile in flight, and of the one after
+  bool bad[2];
+
+  auto fetch = [&](int kt) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bool outside = (unsigned)id[half] >= (unsigned)a.pages;
+      bad[half] = outside;
+      if (outside) id[half] = 0;
+      const int key = kt * BN + half * 16;
+      const long long row = (((long long)id[half] * a.Hk + h)
+                             << a.page_log2) + (key & in_page);
+      const uint8_t* src = kc + (row + col) * (D * EB);
+      if constexpr (Q8) ksr[half] = a.k_scale[row + col];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        if constexpr (KB == 16) {
+          kr[half][i] = *reinterpret_cast<const u4*>(src + i * 64 + grp * 16);
+        } else {
+          u2 x = *reinterpret_cast<const u2*>(src + grp * 8);
+          kr[half][i] = u4{x[0], x[1], 0, 0};
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int vrow = i * VROWS + lane / LPR;
+      const int half = vrow >> 4;
+      const int key = kt * BN + half * 16;
+      const int p = half ? id[1] : id[0];
+      const long long row = (((long long)p * a.Hk + h) << a.page_log2) +
+                            (key & in_page) + (vrow & 15);
+      if constexpr (Q8) vsr[i] = a.v_scale[row];
+      vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
+                                           (lane % LPR) * 16);
+    }
+  };
+
+  f4 o[RT][NT];
+  float m[RT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = minus_inf();
+    sum[rt] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[rt][t] = f4{0, 0, 0, 0};
+  }
+
+  char* mine_v = lds + wave * (BN * D * 2);
+  int kt = mine.first + wave;
+  if (kt < mine.last) {
+    id[0] = page_of(kt * BN);
+    id[1] = page_of(kt * BN + 16);
+    fetch(kt);
+    nid[0] = page_of((kt + WAVES) * BN);
+    nid[1] = page_of((kt + WAVES) * BN + 16);
+  }
+  for (; kt < mine.last; kt += WAVES) {
+    const int key0 = kt * BN;
+    const bool bad0 = bad[0], bad1 = bad[1];
+
+    // S^T: 2 tiles of 16 keys
+    f4 sc[RT][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sc[rt][half] = f4{0, 0, 0, 0};
+      float scale = 1.0f;
+      if constexpr (Q8) scale = scale_of(ksr[half]);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        Oct<K> x;
+        if constexpr (Q8) {
+          const u4 w = kr[half][KB == 16 ? f >> 1 : f];
+          widen(x, (KB == 16 && (f & 1)) ? u2{w[2], w[3]} : u2{w[0], w[1]},
+                scale);
+        } else {
+          x.raw = kr[half][f];
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          sc[rt][half] = mfma16(x.v, q[rt][f].v, sc[rt][half]);
+      }
+    }
+
+    // V to the wave's LDS; rows past the end as 0
+    bool odd_v = false;
+    const bool past = key0 + BN > seen_max;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int vrow = i * VROWS + lane / LPR;
+      const bool there =
+          (!past || key0 + vrow < seen_max) && !(vrow < 16 ? bad0 : bad1);
+      if constexpr (Q8) {
+        const float scale = scale_of(vsr[i]);
+        Oct<K> x, y;
+        widen(x, u2{vr[i][0], vr[i][1]}, scale);
+        widen(y, u2{vr[i][2], vr[i][3]}, scale);
+        if (!there) x.raw = y.raw = u4{0, 0, 0, 0};
+        odd_v |= strange(x) || strange(y);
+        const int c = (lane % LPR) * 2;
+        char* row = mine_v + vrow * (D * 2);
+        *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c + 1) * 16) = y.raw;
+      } else {
+        Oct<K> x;
+        x.raw = there ? vr[i] : u4{0, 0, 0, 0};
+        odd_v |= strange(x);
+        *reinterpret_cast<u4*>(mine_v + vrow * (D * 2) +
+                               few_piece<D>(vrow, lane % LPR) * 16) = x.raw;
+      }
+    }
+    wave_fence();
+
+    // the next tile is on its way while this one's softmax is worked out
+    if (kt + WAVES < mine.last) {
+      id[0] = nid[0];
+      id[1] = nid[1];
+      fetch(kt + WAVES);
+      nid[0] = page_of((kt + 2 * WAVES) * BN);
+      nid[1] = page_of((kt + 2 * WAVES) * BN + 16);
+    }
+
+    const bool cut = key0 + BN > seen_min || bad0 || bad1;
+    Oct<K> p[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x[8];
+      float top = minus_inf();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = sc[rt][j >> 2][j & 3] * a.scale;
+        if (cut) {
+          const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
+          if ((j >> 2) ? bad1 : bad0) x[j] = nan_f32();
+          if (key >= seen[rt]) x[j] = minus_inf();
+        }
+        top = fmaxf(top, x[j]);
+      }
+      top = lane_xor32_max(lane_xor16_max(top));
+      if (__ballot(top > m[rt])) {
+        const float next = fmaxf(m[rt], top);
+        const float keep = exp2_of(m[rt] - base_of(next));
+        m[rt] = next;
+        sum[rt] *= keep;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[rt][t] *= keep;
+      }
+      const float base = base_of(m[rt]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float e = exp2_of(x[j] - base);
+        sum[rt] += e;
+        p[rt].h[j] = (T)e;
+      }
+    }
+
+    // O^T += V^T P^T: step j of a lane's 8 keys is 4 grp + j of the first
+    // 16, then of the last 16
+    auto v_piece = [&](int t) {
+      const int r = grp * 4 + (col >> 2);
+      const int c = t * 2 + ((col >> 1) & 1), within = (col & 1) * 8;
+      u2 lo = transposed(mine_v + r * (D * 2) + few_piece<D>(r, c) * 16 +
+                         within);
+      u2 hi = transposed(mine_v + (r + 16) * (D * 2) +
+                         few_piece<D>(r + 16, c) * 16 + within);
+      Oct<K> x;
+      x.raw = u4{lo[0], lo[1], hi[0], hi[1]};
+      return x;
+    };
+    if (seen_min < seen_max && cut && __ballot(odd_v)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const Oct<K> x = v_piece(t);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          o[rt][t] = mfma16(only<K>(x, 0).v, p[rt].v, o[rt][t]);
+          Oct<K> there;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
+            there.h[j] = (T)(key < seen[rt] ? 1.0f : 0.0f);
+          }
+          for (int kind = 1; kind < 4; ++kind) {
+            f4 hit = mfma16(only<K>(x, kind).v, there.v, f4{0, 0, 0, 0});
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              o[rt][t][j] += hit[j] > 0.0f ? special(kind) : 0.0f;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const Oct<K> x = v_piece(t);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][t] = mfma16(x.v, p[rt].v, o[rt][t]);
+      }
+    }
+    wave_fence();
+  }
+
+  // join the waves, 16 rows at a time
+  float(*all)[16][JS] = reinterpret_cast<float(*)[16][JS]>(lds);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    __syncthreads();
+    const float l = lane_xor32_add(lane_xor16_add(sum[rt]));
+    if (grp == 0) {
+      stat[0][wave][col] = m[rt];
+      stat[1][wave][col] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      *reinterpret_cast<f4*>(&all[wave][col][t * 16 + grp * 4]) = o[rt][t];
+    __syncthreads();
+    const int row = threadIdx.x >> 4, r = s.row0 + rt * 16 + row;
+    if (r >= s.rows) continue;
+    float top = minus_inf();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[0][w][row]);
+    const float base = base_of(top);
+    float keep[WAVES], total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      keep[w] = exp2_of(stat[0][w][row] - base);
+      total += stat[1][w][row] * keep[w];
+    }
+    constexpr int PER = D / 16;
+    const int d0 = (threadIdx.x & 15) * PER;
+    float x[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      x[j] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) x[j] += all[w][row][d0 + j] * keep[w];
+    }
+    if (mine.active == 1) {
+      const int t = r / a.G, g = r % a.G;
+      const bool none = seen_by(a, s, r) == 0;
+      const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
+      T* dst = (T*)a.out + ((long long)(s.q0 + t) * a.Hq + h * a.G + g) * D;
+      T y[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        y[j] = none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
+      __builtin_memcpy(dst + d0, y, sizeof y);
+    } else {
+      float* part = a.parts + (((long long)blockIdx.x * a.splits +
+                                blockIdx.y) * BM + rt * 16 + row) * (D + 2);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) part[d0 + j] = x[j];
+      if ((threadIdx.x & 15) == 0) {
+        part[D] = top;
+        part[D + 1] = total;
+      }
+    }
+  }
+}
+
+// ---- many rows -----------------------------------------------------------
+
+// 16-byte pieces of K rows: 16 neighbouring rows' same piece on different
+// banks; of V rows: 4 neighbouring rows' same 64 bytes
+template <int D>
+__device__ inline int k_piece(int row, int c) {
+  return c ^ ((row / (128 / D)) & (D / 8 - 1));
+}
+template <int D>
+__device__ inline int v_piece_at(int row, int c) {
+  if constexpr (D == 128) return c ^ ((row & 3) << 2);
+  if constexpr (D == 64) return c ^ (((row >> 1) & 1) << 2);
+  return c;
+}
+
+template <typename K, int D, bool Q8>
+__global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
+  typedef typename K::T T;
+  constexpr int BM = 128, BN = 64, WAVES = 4;
+  constexpr int NF = D / 16;            // steps of the product over D
+  constexpr int NT = D / 32;            // tiles of 32 values of O^T
+  constexpr int EB = Q8 ? 1 : 2;
+  constexpr int LPR = D * EB / 16;      // lanes for one row
+  constexpr int ROWS = 256 / LPR;       // rows of one load
+  constexpr int NL = ROWS >= BN ? 1 : BN / ROWS;
+  constexpr int TILE = BN * D * 2;      // bytes of a tile in LDS
+
+  __shared__ __attribute__((aligned(16))) char lds[2][2][TILE];
+  __shared__ int odd_tile[2];  // the last tile here whose V is strange, + 1
+
+  const int h = blockIdx.x % a.Hk;
+  const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
+  const Span s = find(a, tile, BM);
+  if (s.seq < 0) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = lane & 31, hi = lane >> 5;
+
+  const int seen_min = seen_by(a, s, s.row0);
+  const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
+  const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
+                              4);
+  if ((int)blockIdx.y >= mine.active) return;
+  if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+  __syncthreads();
+
+  // this wave's rows
+  const int w0 = s.row0 + wave * 32, r = w0 + col;
+  const bool real = r < s.rows;
+  const int my_t = real ? r / a.G : 0, my_g = real ? r % a.G : 0;
+  const int seen = seen_by(a, s, r);
+  const int wave_min =
+      w0 + 31 < s.rows ? seen_by(a, s, w0) : 0;  // rows past the end see none
+  const int wave_max =
+      w0 < s.rows ? seen_by(a, s, min(w0 + 32, s.rows) - 1) : 0;
+  Oct<K> q[NF];
+  {
+    const T* src = (const T*)a.q + (s.q0 + my_t) * a.q_row +
+                   (long long)(h * a.G + my_g) * a.q_head;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      q[f].raw = real ? *reinterpret_cast<const u4*>(src + f * 16 + hi * 8)
+                      : u4{0, 0, 0, 0};
+  }
+
+  const int* pages = a.table + s.seq * a.table_row;
+  const uint8_t* kc = (const uint8_t*)a.k;
+  const uint8_t* vc = (const uint8_t*)a.v;
+  const int in_page = (1 << a.page_log2) - 1;
+  const int lrow = threadIdx.x / LPR, lpos = threadIdx.x % LPR;
+  const bool loads = lrow < BN;
+
+  u4 kr[NL], vr[NL];
+  uint32_t ksr[NL], vsr[NL];
+  int ids[NL];
+
+  auto look_up = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int key = kt * BN + i * ROWS + lrow;
+      ids[i] = loads && kt < mine.last && key < seen_max
+                   ? pages[key >> a.page_log2] : 0;
+    }
+  };
+  auto fetch = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int id = (unsigned)ids[i] < (unsigned)a.pages ? ids[i] : 0;
+      const int key = kt * BN + i * ROWS + lrow;
+      const long long row = (((long long)id * a.Hk + h) << a.page_log2) +
+                            (key & in_page);
+      if (loads) {
+        kr[i] = *reinterpret_cast<const u4*>(kc + row * (D * EB) + lpos * 16);
+        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) + lpos * 16);
+        if constexpr (Q8) {
+          ksr[i] = a.k_scale[row];
+          vsr[i] = a.v_scale[row];
+        }
+      }
+    }
+  };
+  auto put = [&](int kt) {
+    if (!loads) return;
+    char* kd = lds[kt & 1][0];
+    char* vd = lds[kt & 1][1];
+    const bool past = (kt + 1) * BN > seen_max;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i * ROWS + lrow;
+      // a key without a page scores NaN: its K row is NaN, its V row 0
+      const bool paged = (unsigned)ids[i] < (unsigned)a.pages;
+      const bool there = paged && (!past || kt * BN + row < seen_max);
+      if (!paged) {
+        const uint32_t n = Q8 ? 0x7f7f7f7fu : 0x7fff7fffu;
+        kr[i] = u4{n, n, n, n};
+      }
+      if constexpr (Q8) {
+        Oct<K> x, y;
+        float sc = scale_of(ksr[i]);
+        widen(x, u2{kr[i][0], kr[i][1]}, sc);
+        widen(y, u2{kr[i][2], kr[i][3]}, sc);
+        const int c = lpos * 2;
+        *reinterpret_cast<u4*>(kd + row * (D * 2) + k_piece<D>(row, c) * 16) =
+            x.raw;
+        *reinterpret_cast<u4*>(kd + row * (D * 2) +
+                               k_piece<D>(row, c + 1) * 16) = y.raw;
+        sc = scale_of(vsr[i]);
+        widen(x, u2{vr[i][0], vr[i][1]}, sc);
+        widen(y, u2{vr[i][2], vr[i][3]}, sc);
+        if (!there) x.raw = y.raw = u4{0, 0, 0, 0};
+        odd |= strange(x) || strange(y);
+        *reinterpret_cast<u4*>(vd + row * (D * 2) +
+                               v_piece_at<D>(row, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(vd + row * (D * 2) +
+                               v_piece_at<D>(row, c + 1) * 16) = y.raw;
+      } else {
+        *reinterpret_cast<u4*>(kd + row * (D * 2) +
+                               k_piece<D>(row, lpos) * 16) = kr[i];
+        Oct<K> x;
+        x.raw = there ? vr[i] : u4{0, 0, 0, 0};
+        odd |= strange(x);
+        *reinterpret_cast<u4*>(vd + row * (D * 2) +
+                               v_piece_at<D>(row, lpos) * 16) = x.raw;
+      }
+    }
+    if (odd) odd_tile[kt & 1] = kt + 1;
+  };
+
+  f16v o[NT];
+  float m = minus_inf(), sum = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
+
+  int kt = mine.first;
+  if (kt < mine.last) {
+    look_up(kt);
+    fetch(kt);
+    put(kt);
+  }
+  __syncthreads();
+  for (; kt < mine.last; ++kt) {
+    if (kt + 1 < mine.last) {
+      look_up(kt + 1);
+      fetch(kt + 1);
+    }
+    const int key0 = kt * BN;
+    if (key0 < wave_max) {
+      const char* kd = lds[kt & 1][0];
+      const char* vd = lds[kt & 1][1];
+      f16v sc[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[half][j] = 0.0f;
+        const int row = half * 32 + col;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          Oct<K> x;
+          x.raw = *reinterpret_cast<const u4*>(
+              kd + row * (D * 2) + k_piece<D>(row, f * 2 + hi) * 16);
+          sc[half] = mfma32(x.v, q[f].v, sc[half]);
+        }
+      }
+      const bool cut = key0 + BN > wave_min;
+      float top = minus_inf();
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x = sc[half][j] * a.scale;
+          if (cut) {
+            const int key =
+                key0 + half * 32 + (j & 3) + 8 * (j >> 2) + 4 * hi;
+            if (key >= seen) x = minus_inf();
+          }
+          sc[half][j] = x;
+          top = fmaxf(top, x);
+        }
+      top = lane_xor32_max(top);
+      if (__ballot(top > m)) {
+        const float next = fmaxf(m, top);
+        const float keep = exp2_of(m - base_of(next));
+        m = next;
+        sum *= keep;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[t][j] *= keep;
+      }
+      const float base = base_of(m);
+      Oct<K> p[4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float e = exp2_of(sc[half][j] - base);
+          sum += e;
+          p[half * 2 + (j >> 3)].h[j & 7] = (T)e;
+        }
+      // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
+      const int tr = hi * 4 + ((lane & 15) >> 2);
+      const int tc = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
+      const int within = (lane & 1) * 8;
+      auto v_piece = [&](int step, int t) {
+        const int r0 = step * 16 + tr, c = t * 4 + tc;
+        u2 lo = transposed(vd + r0 * (D * 2) + v_piece_at<D>(r0, c) * 16 +
+                           within);
+        u2 up = transposed(vd + (r0 + 8) * (D * 2) +
+                           v_piece_at<D>(r0 + 8, c) * 16 + within);
+        Oct<K> x;
+        x.raw = u4{lo[0], lo[1], up[0], up[1]};
+        return x;
+      };
+      if (cut && odd_tile[kt & 1] == kt + 1) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          for (int kind = 1; kind < 4; ++kind) {
+            f16v hit;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) hit[j] = 0.0f;
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+              Oct<K> there;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int key = key0 + step * 16 + (j & 3) + 8 * (j >> 2) +
+                                4 * hi;
+                there.h[j] = (T)(key < seen ? 1.0f : 0.0f);
+              }
+              hit = mfma32(only<K>(v_piece(step, t), kind).v, there.v, hit);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              o[t][j] += hit[j] > 0.0f ? special(kind) : 0.0f;
+          }
+#pragma unroll
+          for (int step = 0; step < 4; ++step)
+            o[t] = mfma32(only<K>(v_piece(step, t), 0).v, p[step].v, o[t]);
+        }
+      } else {
+#pragma unroll
+        for (int step = 0; step < 4; ++step)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            o[t] = mfma32(v_piece(step, t).v, p[step].v, o[t]);
+      }
+    }
+    if (kt + 1 < mine.last) put(kt + 1);
+    __syncthreads();
+  }
+
+  sum = lane_xor32_add(sum);
+  if (!real) return;
+  if (mine.active == 1) {
+    const bool none = seen == 0;
+    const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / sum;
+    T* dst = (T*)a.out +
+             ((long long)(s.q0 + my_t) * a.Hq + h * a.G + my_g) * D;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        T y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[i] = none && !s.broken ? (T)0.0f : (T)(o[t][j + i] * inv);
+        __builtin_memcpy(dst + t * 32 + 2 * j + 4 * hi, y, sizeof y);
+      }
+  } else {
+    float* part = a.parts + (((long long)(tile * a.Hk + h) * a.splits +
+                              blockIdx.y) * BM + wave * 32 + col) * (D + 2);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; j += 2)
+        *reinterpret_cast<f2*>(part + t * 32 + (j & 3) + 8 * (j >> 2) +
+                               4 * hi) = f2{o[t][j], o[t][j + 1]};
+    if (hi == 0) {
+      part[D] = m;
+      part[D + 1] = sum;
+    }
+  }
+}
+
+// ---- the splits' parts ------------------------------------------------------
+
+// One workgroup for 4 rows of a tile; a wave adds up one row.
+template <typename K, int D>
+__global__ void __launch_bounds__(256)
+join_kernel(Args a, int BM, int BN, int least) {
+  typedef typename K::T T;
+  const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
+  const Span s = find(a, tile, BM);
+  if (s.seq < 0) return;
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int r = s.row0 + row, lane = threadIdx.x & 63;
+  if (r >= s.rows) return;
+  const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
+  const Share all = share_of((seen_max + BN - 1) / BN, a.splits, 0, least);
+  if (all.active == 1) return;
+  const float* part =
+      a.parts + ((long long)blockIdx.x * a.splits * BM + row) * (D + 2);
+  const long long step = (long long)BM * (D + 2);
+  float top = minus_inf();
+  for (int i = lane; i < all.active; i += 64)
+    top = fmaxf(top, part[i * step + D]);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+  const float base = base_of(top);
+  constexpr int PER = D >= 64 ? D / 64 : 1;
+  const bool works = lane * PER < D;
+  float x[PER] = {}, total = 0.0f;
+  for (int i = 0; i < all.active; ++i) {
+    const float* at = part + i * step;
+    const float keep = exp2_of(at[D] - base);
+    total += at[D + 1] * keep;
+    if (works)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) x[j] += at[lane * PER + j] * keep;
+  }
+  if (!works) return;
+  const bool none = seen_by(a, s, r) == 0;
+  const float inv = s.broken ? nan_f32() : 1.0f / total;
+  T* dst = (T*)a.out +
+           ((long long)(s.q0 + r / a.G) * a.Hq + h * a.G + r % a.G) * D;
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    dst[lane * PER + j] =
+        none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
+}
+
+// ---- launching ------------------------------------------------------------
+
+template <typename K, int D>
+int launch_join(Args& a, int tiles, int BM, int BN, int least,
+                hipStream_t stream) {
+  if (a.splits == 1) return 0;
+  void* args[] = {&a, &BM, &BN, &least};
+  return (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&join_kernel<K, D>),
+      dim3(tiles * a.Hk, BM / 4), dim3(256), args, 0, stream);
+}
+
+template <typename K, int D, bool Q8, int RT>
+int launch_few(Args& a, int tiles, hipStream_t stream) {
+  void* args[] = {&a};
+  int rc = (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&few_kernel<K, D, Q8, RT>),
+      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
+  return rc ? rc : launch_join<K, D>(a, tiles, 16 * RT, 32, 8, stream);
+}
+
+template <typename K, int D, bool Q8>
+int launch_many(Args& a, int tiles, hipStream_t stream) {
+  void* args[] = {&a, &tiles};
+  int rc = (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
+      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
+  return rc ? rc : launch_join<K, D>(a, tiles, 128, 64, 4, stream);
+}
+
+// rows of a tile of the few kernel: 16, 32, or 0 for none; the same for
+// many: whether it runs. Both run where the batch may hold either kind.
+struct Plan {
+  int few_rows, few_splits, many, many_splits;
+};
+
+template <typename K, int D, bool Q8>
+int run(Args a, const Plan& p, hipStream_t stream) {
+  int rc = 0;
+  if (p.few_rows) {
+    a.which = p.many ? 1 : 0;
+    a.splits = p.few_splits;
+    const int tiles =
+        p.many ? a.B : (int)((long long)a.T * a.G / p.few_rows) + a.B;
+    rc = p.few_rows == 16 ? launch_few<K, D, Q8, 1>(a, tiles, stream)
+                          : launch_few<K, D, Q8, 2>(a, tiles, stream);
+  }
+  if (!rc && p.many) {
+    a.which = p.few_rows ? 2 : 0;
+    a.splits = p.many_splits;
+    const int tiles = (int)((long long)a.T * a.G / 128) + a.B;
+    rc = launch_many<K, D, Q8>(a, tiles, stream);
+  }
+  return rc;
+}
+
+template <typename K, bool Q8>
+int run_d(const Args& a, const Plan& p, int D, hipStream_t stream) {
+  switch (D) {
+    case 32: return run<K, 32, Q8>(a, p, stream);
+    case 64: return run<K, 64, Q8>(a, p, stream);
+    case 128: return run<K, 128, Q8>(a, p, stream);
+  }
+  return (int)hipErrorInvalidValue;
+}
+
+}  // namespace
+
+extern "C" {
+
+// parts: 32-bit floats, for each kernel that splits tiles * Hk * splits *
+// rows of a tile * (D + 2) of them; the two kernels use the same ones, one
+// after the other.
+int tf_paged_attention(
+    const void* q, const void* k, const void* v, const void* k_scale,
+    const void* v_scale, const void* q_starts, const void* kv_lens,
+    const void* table, void* out, void* parts, long long q_row,
+    long long q_head, long long table_row, int cols, int T, int B, int Hq,
+    int Hk, int pages, int page_log2, int D, float scale, int causal,
+    int fp16, int few_rows, int few_splits, int many, int many_splits,
+    void* stream) {
+  if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || cols < 0 ||
+      pages < 1 || page_log2 < 4 || page_log2 > 10 ||
+      (few_rows != 0 && few_rows != 16 && few_rows != 32) ||
+      (many && few_rows == 16) || (!many && !few_rows) || few_splits < 1 ||
+      few_splits > 65535 || many_splits < 1 || many_splits > 65535 ||
+      ((few_splits > 1 || many_splits > 1) && !parts) ||
+      ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
+      (long long)T * (Hq / Hk) >= (1LL << 31))
+    return (int)hipErrorInvalidValue;
+  Args a{q, k, v, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
+         (const int*)q_starts, (const int*)kv_lens, (const int*)table, out,
+         (float*)parts, q_row, q_head, table_row, cols, T, B, Hq, Hk,
+         Hq / Hk, pages, page_log2, scale * 1.4426950408889634f, causal, 1,
+         0};
+  const Plan p{few_rows, few_splits, many, many_splits};
+  const bool q8 = k_scale != nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  return fp16 ? (q8 ? run_d<Fp16, true>(a, p, D, st)
+                    : run_d<Fp16, false>(a, p, D, st))
+              : (q8 ? run_d<Bf16, true>(a, p, D, st)
+                    : run_d<Bf16, false>(a, p, D, st));
+}
+
+}  // extern "C"
