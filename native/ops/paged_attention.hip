@@ -136,6 +136,12 @@ __device__ inline Share share_of(int all, int splits, int split, int least) {
   return s;
 }
 
+// a load by the scalar unit: the address is the wave's, and nothing in the
+// kernel writes there. It is not counted with the vector loads in flight.
+__device__ inline int uniform_load(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)(uintptr_t)p;
+}
+
 // ---- small pieces ------------------------------------------------------
 
 __device__ inline float lane_xor16_max(float x) {
@@ -178,6 +184,18 @@ __device__ inline f16v mfma32(Bf16::V8 a, Bf16::V8 b, f16v c) {
 }
 __device__ inline f16v mfma32(Fp16::V8 a, Fp16::V8 b, f16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// sum + the two values of pair j: what is summed is what is multiplied
+__device__ inline float add_pair(const Oct<Bf16>& p, int j, float sum) {
+  const Bf16::V2 one = {(__bf16)1.0f, (__bf16)1.0f};
+  return __builtin_amdgcn_fdot2_f32_bf16(Bf16::V2{p.v[2 * j], p.v[2 * j + 1]},
+                                         one, sum, false);
+}
+__device__ inline float add_pair(const Oct<Fp16>& p, int j, float sum) {
+  const Fp16::V2 one = {(_Float16)1.0f, (_Float16)1.0f};
+  return __builtin_amdgcn_fdot2(Fp16::V2{p.v[2 * j], p.v[2 * j + 1]}, one,
+                                sum, false);
 }
 
 // 8 codes times their scale, rounded to 16 bits: exact, but for fp16 where
@@ -612,6 +630,25 @@ __device__ inline int v_piece_at(int row, int c) {
   return c;
 }
 
+// 16 bytes a lane from memory to LDS, at `to` + 16 * lane, without a register
+// between; `base` and `to` are the wave's, `off` the lane's. Nothing but
+// landed() waits for it.
+__device__ inline void to_lds(const void* base, uint32_t off, uint32_t to) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(off), "s"(base), "s"(to)
+      : "memory");
+}
+__device__ inline void landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+__device__ inline uint32_t lds_address(const void* p) {
+  return (uint32_t)(size_t)(const __attribute__((address_space(3))) char*)p;
+}
+
 template <typename K, int D, bool Q8>
 __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   typedef typename K::T T;
@@ -620,18 +657,20 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   constexpr int NT = D / 32;            // tiles of 32 values of O^T
   constexpr int EB = Q8 ? 1 : 2;
   constexpr int LPR = D * EB / 16;      // lanes for one row
-  constexpr int ROWS = 256 / LPR;       // rows of one load
-  constexpr int NL = ROWS >= BN ? 1 : BN / ROWS;
+  constexpr int ROWS = 64 / LPR;        // rows of one load of a wave
+  constexpr int NL = ROWS >= 16 ? 1 : 16 / ROWS;  // loads for its 16 rows
   constexpr int TILE = BN * D * 2;      // bytes of a tile in LDS
 
-  __shared__ __attribute__((aligned(16))) char lds[2][2][TILE];
+  // K, V of one tile, then of the next
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   __shared__ int odd_tile[2];  // the last tile here whose V is strange, + 1
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
   const Span s = find(a, tile, BM);
   if (s.seq < 0) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int col = lane & 31, hi = lane >> 5;
 
   const int seen_min = seen_by(a, s, s.row0);
@@ -656,90 +695,111 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
     const T* src = (const T*)a.q + (s.q0 + my_t) * a.q_row +
                    (long long)(h * a.G + my_g) * a.q_head;
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
+    for (int f = 0; f < NF; ++f) {
       q[f].raw = real ? *reinterpret_cast<const u4*>(src + f * 16 + hi * 8)
                       : u4{0, 0, 0, 0};
+      // scores grow with the product below: a negative scale turns q
+      if (a.scale < 0.0f) q[f].raw ^= u4{0x80008000u, 0x80008000u,
+                                         0x80008000u, 0x80008000u};
+    }
   }
+  const float scale = fabsf(a.scale);
 
+  // Wave w brings keys 16 w .. 16 w + 15 of a tile: they lie in one page.
   const int* pages = a.table + s.seq * a.table_row;
-  const uint8_t* kc = (const uint8_t*)a.k;
-  const uint8_t* vc = (const uint8_t*)a.v;
   const int in_page = (1 << a.page_log2) - 1;
-  const int lrow = threadIdx.x / LPR, lpos = threadIdx.x % LPR;
-  const bool loads = lrow < BN;
-
-  u4 kr[NL], vr[NL];
+  const int lrow = lane / LPR, lpos = lane % LPR;
+  auto page_of = [&](int kt) {
+    const int key = kt * BN + wave * 16;
+    return kt < mine.last && key < seen_max
+               ? uniform_load(pages + (key >> a.page_log2)) : 0;
+  };
+  uint32_t k_off[NL], v_off[NL];  // 16 bits: what a lane brings of 16 rows
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int row = i * ROWS + lrow;
+    k_off[i] = row * (D * 2) + k_piece<D>(wave * 16 + row, lpos) * 16;
+    v_off[i] = row * (D * 2) + v_piece_at<D>(wave * 16 + row, lpos) * 16;
+  }
+  u4 kr[NL], vr[NL];  // 8 bits: codes on their way
   uint32_t ksr[NL], vsr[NL];
-  int ids[NL];
+  const bool loads = lrow < 16;
+  const uint32_t lds0 = lds_address(lds);
+  int id = 0, bad = 0;
 
-  auto look_up = [&](int kt) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int key = kt * BN + i * ROWS + lrow;
-      ids[i] = loads && kt < mine.last && key < seen_max
-                   ? pages[key >> a.page_log2] : 0;
-    }
-  };
   auto fetch = [&](int kt) {
+    bad = (unsigned)id >= (unsigned)a.pages;
+    const int key = kt * BN + wave * 16;
+    const long long row =
+        (((long long)(bad ? 0 : id) * a.Hk + h) << a.page_log2) +
+        (key & in_page);
+    const char* ks = (const char*)a.k + row * (D * EB);
+    const char* vs = (const char*)a.v + row * (D * EB);
+    if constexpr (Q8) {
+      if (loads)
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int id = (unsigned)ids[i] < (unsigned)a.pages ? ids[i] : 0;
-      const int key = kt * BN + i * ROWS + lrow;
-      const long long row = (((long long)id * a.Hk + h) << a.page_log2) +
-                            (key & in_page);
-      if (loads) {
-        kr[i] = *reinterpret_cast<const u4*>(kc + row * (D * EB) + lpos * 16);
-        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) + lpos * 16);
-        if constexpr (Q8) {
-          ksr[i] = a.k_scale[row];
-          vsr[i] = a.v_scale[row];
+        for (int i = 0; i < NL; ++i) {
+          const int at = i * ROWS + lrow;
+          kr[i] = *reinterpret_cast<const u4*>(ks + at * D + lpos * 16);
+          vr[i] = *reinterpret_cast<const u4*>(vs + at * D + lpos * 16);
+          ksr[i] = a.k_scale[row + at];
+          vsr[i] = a.v_scale[row + at];
         }
-      }
+    } else {
+      const uint32_t to = lds0 + (kt & 1) * (2 * TILE) + wave * (TILE / 4);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) to_lds(ks, k_off[i], to + i * 1024);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) to_lds(vs, v_off[i], to + TILE + i * 1024);
     }
   };
+  // what fetch brought becomes the tile, but for the barrier
   auto put = [&](int kt) {
-    if (!loads) return;
-    char* kd = lds[kt & 1][0];
-    char* vd = lds[kt & 1][1];
-    const bool past = (kt + 1) * BN > seen_max;
+    char* kd = lds + (kt & 1) * (2 * TILE) + wave * (TILE / 4);
+    char* vd = kd + TILE;
+    const int key0 = kt * BN + wave * 16;
+    const bool past = key0 + 16 > seen_max;
+    const bool cut = (kt + 1) * BN > seen_min;
     bool odd = false;
+    if constexpr (Q8) {
+      if (!loads) return;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = i * ROWS + lrow;
-      // a key without a page scores NaN: its K row is NaN, its V row 0
-      const bool paged = (unsigned)ids[i] < (unsigned)a.pages;
-      const bool there = paged && (!past || kt * BN + row < seen_max);
-      if (!paged) {
-        const uint32_t n = Q8 ? 0x7f7f7f7fu : 0x7fff7fffu;
-        kr[i] = u4{n, n, n, n};
-      }
-      if constexpr (Q8) {
+      for (int i = 0; i < NL; ++i) {
+        const int row = i * ROWS + lrow, c = lpos * 2;
+        const bool there = !bad && (!past || key0 + row < seen_max);
+        // a key without a page scores NaN: its K row is NaN, its V row 0
+        if (bad) kr[i] = u4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu,
+                            0x7f7f7f7fu};
         Oct<K> x, y;
         float sc = scale_of(ksr[i]);
         widen(x, u2{kr[i][0], kr[i][1]}, sc);
         widen(y, u2{kr[i][2], kr[i][3]}, sc);
-        const int c = lpos * 2;
-        *reinterpret_cast<u4*>(kd + row * (D * 2) + k_piece<D>(row, c) * 16) =
-            x.raw;
-        *reinterpret_cast<u4*>(kd + row * (D * 2) +
-                               k_piece<D>(row, c + 1) * 16) = y.raw;
+        char* to = kd + row * (D * 2);
+        const int at = wave * 16 + row;
+        *reinterpret_cast<u4*>(to + k_piece<D>(at, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(to + k_piece<D>(at, c + 1) * 16) = y.raw;
         sc = scale_of(vsr[i]);
         widen(x, u2{vr[i][0], vr[i][1]}, sc);
         widen(y, u2{vr[i][2], vr[i][3]}, sc);
         if (!there) x.raw = y.raw = u4{0, 0, 0, 0};
         odd |= strange(x) || strange(y);
-        *reinterpret_cast<u4*>(vd + row * (D * 2) +
-                               v_piece_at<D>(row, c) * 16) = x.raw;
-        *reinterpret_cast<u4*>(vd + row * (D * 2) +
-                               v_piece_at<D>(row, c + 1) * 16) = y.raw;
-      } else {
-        *reinterpret_cast<u4*>(kd + row * (D * 2) +
-                               k_piece<D>(row, lpos) * 16) = kr[i];
-        Oct<K> x;
-        x.raw = there ? vr[i] : u4{0, 0, 0, 0};
-        odd |= strange(x);
-        *reinterpret_cast<u4*>(vd + row * (D * 2) +
-                               v_piece_at<D>(row, lpos) * 16) = x.raw;
+        to = vd + row * (D * 2);
+        *reinterpret_cast<u4*>(to + v_piece_at<D>(at, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(to + v_piece_at<D>(at, c + 1) * 16) = y.raw;
+      }
+    } else {
+      landed();
+      if (!bad && !cut) return;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        Oct<K>* x = reinterpret_cast<Oct<K>*>(vd + i * 1024 + lane * 16);
+        if (bad || (past && key0 + i * ROWS + lrow >= seen_max))
+          x->raw = u4{0, 0, 0, 0};
+        else
+          odd |= strange(*x);
+        if (bad)
+          *reinterpret_cast<u4*>(kd + i * 1024 + lane * 16) =
+              u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
       }
     }
     if (odd) odd_tile[kt & 1] = kt + 1;
@@ -752,53 +812,70 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
 
+  // a lane's places in a tile: of K the row `col`, of V the 4 keys by 4
+  // values of its transposing reads
+  uint32_t k_at[NF], v_at[NT];
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+    k_at[f] = col * (D * 2) + k_piece<D>(col, f * 2 + hi) * 16;
+  {
+    const int row = hi * 4 + ((lane & 15) >> 2);
+    const int c = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      v_at[t] = row * (D * 2) + v_piece_at<D>(row, t * 4 + c) * 16 +
+                (lane & 1) * 8;
+  }
+
   int kt = mine.first;
+  id = page_of(kt);
   if (kt < mine.last) {
-    look_up(kt);
     fetch(kt);
+    id = page_of(kt + 1);
     put(kt);
   }
   __syncthreads();
   for (; kt < mine.last; ++kt) {
-    if (kt + 1 < mine.last) {
-      look_up(kt + 1);
+    const bool more = kt + 1 < mine.last;
+    if (more) {
       fetch(kt + 1);
+      id = page_of(kt + 2);
     }
     const int key0 = kt * BN;
     if (key0 < wave_max) {
-      const char* kd = lds[kt & 1][0];
-      const char* vd = lds[kt & 1][1];
+      const char* kd = lds + (kt & 1) * (2 * TILE);
+      const char* vd = kd + TILE;
       f16v sc[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) sc[half][j] = 0.0f;
-        const int row = half * 32 + col;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
           Oct<K> x;
-          x.raw = *reinterpret_cast<const u4*>(
-              kd + row * (D * 2) + k_piece<D>(row, f * 2 + hi) * 16);
+          x.raw = *reinterpret_cast<const u4*>(kd + k_at[f] +
+                                               half * 32 * (D * 2));
           sc[half] = mfma32(x.v, q[f].v, sc[half]);
         }
       }
       const bool cut = key0 + BN > wave_min;
-      float top = minus_inf();
+      if (cut) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float x = sc[half][j] * a.scale;
-          if (cut) {
+          for (int j = 0; j < 16; ++j) {
             const int key =
                 key0 + half * 32 + (j & 3) + 8 * (j >> 2) + 4 * hi;
-            if (key >= seen) x = minus_inf();
+            if (key >= seen) sc[half][j] = minus_inf();
           }
-          sc[half][j] = x;
-          top = fmaxf(top, x);
-        }
-      top = lane_xor32_max(top);
-      if (__ballot(top > m)) {
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) top = fmaxf(top, sc[j >> 4][j & 15]);
+      top = lane_xor32_max(top) * scale;
+      // The sums stay under an old maximum until a score is 2^8 above it:
+      // p is then at most 2^8, with the same relative rounding.
+      if (__ballot(top > m + 8.0f)) {
         const float next = fmaxf(m, top);
         const float keep = exp2_of(m - base_of(next));
         m = next;
@@ -811,23 +888,16 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
       const float base = base_of(m);
       Oct<K> p[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int j = 0; j < 32; ++j)
+        p[j >> 3].h[j & 7] = (T)exp2_of(
+            __builtin_fmaf(sc[j >> 4][j & 15], scale, -base));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float e = exp2_of(sc[half][j] - base);
-          sum += e;
-          p[half * 2 + (j >> 3)].h[j & 7] = (T)e;
-        }
+      for (int j = 0; j < 16; ++j)
+        sum = add_pair(p[j >> 2], j & 3, sum);
       // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
-      const int tr = hi * 4 + ((lane & 15) >> 2);
-      const int tc = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
-      const int within = (lane & 1) * 8;
       auto v_piece = [&](int step, int t) {
-        const int r0 = step * 16 + tr, c = t * 4 + tc;
-        u2 lo = transposed(vd + r0 * (D * 2) + v_piece_at<D>(r0, c) * 16 +
-                           within);
-        u2 up = transposed(vd + (r0 + 8) * (D * 2) +
-                           v_piece_at<D>(r0 + 8, c) * 16 + within);
+        const char* at = vd + v_at[t] + step * 16 * (D * 2);
+        u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
         Oct<K> x;
         x.raw = u4{lo[0], lo[1], up[0], up[1]};
         return x;
@@ -866,7 +936,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
             o[t] = mfma32(v_piece(step, t).v, p[step].v, o[t]);
       }
     }
-    if (kt + 1 < mine.last) put(kt + 1);
+    if (more) put(kt + 1);
     __syncthreads();
   }
 
@@ -1043,8 +1113,9 @@ int tf_paged_attention(
   Args a{q, k, v, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
          (const int*)q_starts, (const int*)kv_lens, (const int*)table, out,
          (float*)parts, q_row, q_head, table_row, cols, T, B, Hq, Hk,
-         Hq / Hk, pages, page_log2, scale * 1.4426950408889634f, causal, 1,
-         0};
+         Hq / Hk, pages, page_log2,
+         // 0 times a masked score would be NaN; this leaves every p 1 too
+         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 0};
   const Plan p{few_rows, few_splits, many, many_splits};
   const bool q8 = k_scale != nullptr;
   hipStream_t st = (hipStream_t)stream;
