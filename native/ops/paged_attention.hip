@@ -54,7 +54,8 @@ struct Args {
   const int* kv_lens;
   const int* table;
   void* out;
-  float* parts;  // [tile * Hk + h][split][row]: D sums, then maximum and sum
+  float* parts;         // [tile * Hk + h][split][row][D]: sums over p v
+  float* stats;         // [tile * Hk + h][split][row][2]: maximum, sum of p
   long long q_row, q_head, table_row;
   int cols;  // of the table
   int T, B, Hq, Hk, G, pages, page_log2;
@@ -240,24 +241,32 @@ __device__ inline bool strange(const Oct<Fp16>& o) {
   return s;
 }
 
-// V's values for the tiles that hold NaN or infinities: the finite ones
-// (kind 0), or 1 where a value is NaN, +inf, -inf (kinds 1, 2, 3)
+// its values, with 0 for those
 template <typename K>
-__device__ inline Oct<K> only(Oct<K> o, int kind) {
+__device__ inline u4 finite_only(Oct<K> o) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float x = (float)o.h[j];
-    bool finite = fabsf(x) < plus_inf();
-    float y = kind == 0   ? (finite ? x : 0.0f)
-              : kind == 1 ? (x != x ? 1.0f : 0.0f)
-              : kind == 2 ? (x == plus_inf() ? 1.0f : 0.0f)
-                          : (x == minus_inf() ? 1.0f : 0.0f);
-    o.h[j] = (typename K::T)y;
-  }
-  return o;
+  for (int j = 0; j < 8; ++j)
+    if (!(fabsf((float)o.h[j]) < plus_inf())) o.h[j] = (typename K::T)0.0f;
+  return o.raw;
 }
-__device__ inline float special(int kind) {
-  return kind == 1 ? nan_f32() : kind == 2 ? plus_inf() : minus_inf();
+
+// Calls add(d, v) for each value v = row[d] of a key's V row in LDS that is
+// NaN or infinite, d and v the wave's. place(d): where value d lies.
+template <typename K, int D, typename P, typename F>
+__device__ inline void each_strange(P place, F add) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int d0 = 0; d0 < D; d0 += 64) {
+    const int d = d0 + lane;
+    float v = d < D ? (float)*place(d) : 0.0f;
+    unsigned long long found = __ballot(!(fabsf(v) < plus_inf()));
+    while (found) {
+      const int i = __ffsll(found) - 1;
+      found &= found - 1;
+      add(d0 + i, __uint_as_float(__builtin_amdgcn_readlane(
+                      __float_as_uint(v), i)));
+    }
+  }
 }
 
 typedef __attribute__((address_space(3))) s4* lds_s4;
@@ -289,7 +298,8 @@ __device__ inline int few_piece(int row, int c) {
 }
 
 template <typename K, int D, bool Q8, int RT>
-__global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
+__global__ void __launch_bounds__(256, Q8 && RT == 1 ? 3 : 2)
+few_kernel(Args a) {
   typedef typename K::T T;
   constexpr int BM = 16 * RT, BN = 32, WAVES = 4;
   constexpr int NF = D / 32;              // steps of the product over D
@@ -311,7 +321,8 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
   const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
   const Span s = find(a, tile, BM);
   if (s.seq < 0) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int col = lane & 15, grp = lane >> 4;
 
   const int seen_min = seen_by(a, s, s.row0);
@@ -338,57 +349,68 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
                                     : 32 * f + grp * 8;
       q[rt][f].raw = real ? *reinterpret_cast<const u4*>(src + d0)
                           : u4{0, 0, 0, 0};
+      // scores grow with the product below: a negative scale turns q
+      if (a.scale < 0.0f) q[rt][f].raw ^= u4{0x80008000u, 0x80008000u,
+                                             0x80008000u, 0x80008000u};
     }
   }
+  const float scale = fabsf(a.scale);
 
   const int* pages = a.table + s.seq * a.table_row;
   const uint8_t* kc = (const uint8_t*)a.k;
   const uint8_t* vc = (const uint8_t*)a.v;
   const int in_page = (1 << a.page_log2) - 1;
 
-  // pages of the two halves of tile kt; keys past the last are not looked up
+  // the page of 16 keys; those past the last are not looked up
   auto page_of = [&](int key) {
-    int p = key < seen_max ? pages[key >> a.page_log2] : 0;
-    return p;
+    return key < seen_max ? uniform_load(pages + (key >> a.page_log2)) : 0;
   };
 
   u4 kr[2][NK], vr[NV];
   uint32_t ksr[2], vsr[NV];
-  int id[2], nid[2];  // of the tile in flight, and of the one after
-  bool bad[2];
+  int id[2];  // pages of the tile to come
+  bool bad0 = false, bad1 = false;
+  const uint32_t k_off = col * (D * EB) + grp * KB;
+  const uint32_t v_off = lane * 16;
 
   auto fetch = [&](int kt) {
+    bad0 = (unsigned)id[0] >= (unsigned)a.pages;
+    bad1 = (unsigned)id[1] >= (unsigned)a.pages;
+    const int key = kt * BN;
+    const long long row0 = (((long long)(bad0 ? 0 : id[0]) * a.Hk + h)
+                            << a.page_log2) + (key & in_page);
+    const long long row1 = (((long long)(bad1 ? 0 : id[1]) * a.Hk + h)
+                            << a.page_log2) + ((key + 16) & in_page);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const bool outside = (unsigned)id[half] >= (unsigned)a.pages;
-      bad[half] = outside;
-      if (outside) id[half] = 0;
-      const int key = kt * BN + half * 16;
-      const long long row = (((long long)id[half] * a.Hk + h)
-                             << a.page_log2) + (key & in_page);
-      const uint8_t* src = kc + (row + col) * (D * EB);
-      if constexpr (Q8) ksr[half] = a.k_scale[row + col];
+      const long long row = half ? row1 : row0;
+      const uint8_t* src = kc + row * (D * EB);
+      if constexpr (Q8) ksr[half] = (a.k_scale + row)[col];
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         if constexpr (KB == 16) {
-          kr[half][i] = *reinterpret_cast<const u4*>(src + i * 64 + grp * 16);
+          kr[half][i] = *reinterpret_cast<const u4*>(src + k_off + i * 64);
         } else {
-          u2 x = *reinterpret_cast<const u2*>(src + grp * 8);
+          u2 x = *reinterpret_cast<const u2*>(src + k_off);
           kr[half][i] = u4{x[0], x[1], 0, 0};
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int vrow = i * VROWS + lane / LPR;
-      const int half = vrow >> 4;
-      const int key = kt * BN + half * 16;
-      const int p = half ? id[1] : id[0];
-      const long long row = (((long long)p * a.Hk + h) << a.page_log2) +
-                            (key & in_page) + (vrow & 15);
-      if constexpr (Q8) vsr[i] = a.v_scale[row];
-      vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
-                                           (lane % LPR) * 16);
+      if constexpr (VROWS <= 16) {
+        constexpr int PER16 = 16 / (VROWS > 16 ? 16 : VROWS);
+        const long long row =
+            (i / PER16 ? row1 : row0) + (i % PER16) * VROWS;
+        if constexpr (Q8) vsr[i] = (a.v_scale + row)[lane / LPR];
+        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) + v_off);
+      } else {  // one load takes both halves
+        const int vrow = lane / LPR;
+        const long long row = (vrow < 16 ? row0 : row1) + (vrow & 15);
+        if constexpr (Q8) vsr[i] = a.v_scale[row];
+        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
+                                             (lane % LPR) * 16);
+      }
     }
   };
 
@@ -403,17 +425,26 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
   }
 
   char* mine_v = lds + wave * (BN * D * 2);
+  uint32_t v_at[NT];  // a lane's 4 keys by 4 values of transposing reads
+  {
+    const int row = grp * 4 + (col >> 2);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      v_at[t] = row * (D * 2) +
+                few_piece<D>(row, t * 2 + ((col >> 1) & 1)) * 16 +
+                (col & 1) * 8;
+  }
   int kt = mine.first + wave;
   if (kt < mine.last) {
     id[0] = page_of(kt * BN);
     id[1] = page_of(kt * BN + 16);
     fetch(kt);
-    nid[0] = page_of((kt + WAVES) * BN);
-    nid[1] = page_of((kt + WAVES) * BN + 16);
+    id[0] = page_of((kt + WAVES) * BN);
+    id[1] = page_of((kt + WAVES) * BN + 16);
   }
   for (; kt < mine.last; kt += WAVES) {
     const int key0 = kt * BN;
-    const bool bad0 = bad[0], bad1 = bad[1];
+    const bool none0 = bad0, none1 = bad1;  // halves without a page
 
     // S^T: 2 tiles of 16 keys
     f4 sc[RT][2];
@@ -439,29 +470,34 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
       }
     }
 
-    // V to the wave's LDS; rows past the end as 0
+    // V to the wave's LDS; rows past the end, or without a page, as 0
+    const bool past = key0 + BN > seen_max || none0 || none1;
+    const bool cut = key0 + BN > seen_min || none0 || none1;
+    const bool look = cut && seen_min < seen_max;
     bool odd_v = false;
-    const bool past = key0 + BN > seen_max;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vrow = i * VROWS + lane / LPR;
-      const bool there =
-          (!past || key0 + vrow < seen_max) && !(vrow < 16 ? bad0 : bad1);
+      if (past) {
+        if (key0 + vrow >= seen_max || (vrow < 16 ? none0 : none1)) {
+          vr[i] = u4{0, 0, 0, 0};
+          vsr[i] = 127;
+        }
+      }
       if constexpr (Q8) {
         const float scale = scale_of(vsr[i]);
         Oct<K> x, y;
         widen(x, u2{vr[i][0], vr[i][1]}, scale);
         widen(y, u2{vr[i][2], vr[i][3]}, scale);
-        if (!there) x.raw = y.raw = u4{0, 0, 0, 0};
-        odd_v |= strange(x) || strange(y);
+        if (look) odd_v |= strange(x) || strange(y);
         const int c = (lane % LPR) * 2;
         char* row = mine_v + vrow * (D * 2);
         *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c) * 16) = x.raw;
         *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c + 1) * 16) = y.raw;
       } else {
         Oct<K> x;
-        x.raw = there ? vr[i] : u4{0, 0, 0, 0};
-        odd_v |= strange(x);
+        x.raw = vr[i];
+        if (look) odd_v |= strange(x);
         *reinterpret_cast<u4*>(mine_v + vrow * (D * 2) +
                                few_piece<D>(vrow, lane % LPR) * 16) = x.raw;
       }
@@ -470,31 +506,28 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
 
     // the next tile is on its way while this one's softmax is worked out
     if (kt + WAVES < mine.last) {
-      id[0] = nid[0];
-      id[1] = nid[1];
       fetch(kt + WAVES);
-      nid[0] = page_of((kt + 2 * WAVES) * BN);
-      nid[1] = page_of((kt + 2 * WAVES) * BN + 16);
+      id[0] = page_of((kt + 2 * WAVES) * BN);
+      id[1] = page_of((kt + 2 * WAVES) * BN + 16);
     }
 
-    const bool cut = key0 + BN > seen_min || bad0 || bad1;
     Oct<K> p[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[8];
-      float top = minus_inf();
+      if (cut) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = sc[rt][j >> 2][j & 3] * a.scale;
-        if (cut) {
+        for (int j = 0; j < 8; ++j) {
           const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
-          if ((j >> 2) ? bad1 : bad0) x[j] = nan_f32();
-          if (key >= seen[rt]) x[j] = minus_inf();
+          if ((j >> 2) ? none1 : none0) sc[rt][j >> 2][j & 3] = nan_f32();
+          if (key >= seen[rt]) sc[rt][j >> 2][j & 3] = minus_inf();
         }
-        top = fmaxf(top, x[j]);
       }
-      top = lane_xor32_max(lane_xor16_max(top));
-      if (__ballot(top > m[rt])) {
+      float top = sc[rt][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[rt][j >> 2][j & 3]);
+      top = lane_xor32_max(lane_xor16_max(top)) * scale;
+      // as in the other kernel, the maximum moves by steps of 2^8 or more
+      if (__ballot(top > m[rt] + 8.0f)) {
         const float next = fmaxf(m[rt], top);
         const float keep = exp2_of(m[rt] - base_of(next));
         m[rt] = next;
@@ -504,55 +537,51 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
       }
       const float base = base_of(m[rt]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float e = exp2_of(x[j] - base);
-        sum[rt] += e;
-        p[rt].h[j] = (T)e;
+      for (int j = 0; j < 8; ++j)
+        p[rt].h[j] = (T)exp2_of(
+            __builtin_fmaf(sc[rt][j >> 2][j & 3], scale, -base));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[rt] = add_pair(p[rt], j, sum[rt]);
+    }
+
+    if (look && __ballot(odd_v)) {
+      // what is not finite goes to the rows that see it, then gives way
+#pragma unroll 1
+      for (int key = 0; key < BN; ++key)
+        each_strange<K, D>(
+            [&](int d) {
+              return (const T*)(mine_v + key * (D * 2) +
+                                few_piece<D>(key, d >> 3) * 16 + (d & 7) * 2);
+            },
+            [&](int d, float v) {
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < NT * 4; ++i)
+                  if (d == (i >> 2) * 16 + grp * 4 + (i & 3) &&
+                      key0 + key < seen[rt])
+                    o[rt][i >> 2][i & 3] += v;
+            });
+      wave_fence();
+#pragma unroll 1
+      for (int i = lane; i < BN * D / 8; i += 64) {
+        Oct<K>* x = reinterpret_cast<Oct<K>*>(mine_v + i * 16);
+        x->raw = finite_only<K>(*x);
       }
+      wave_fence();
     }
 
     // O^T += V^T P^T: step j of a lane's 8 keys is 4 grp + j of the first
     // 16, then of the last 16
-    auto v_piece = [&](int t) {
-      const int r = grp * 4 + (col >> 2);
-      const int c = t * 2 + ((col >> 1) & 1), within = (col & 1) * 8;
-      u2 lo = transposed(mine_v + r * (D * 2) + few_piece<D>(r, c) * 16 +
-                         within);
-      u2 hi = transposed(mine_v + (r + 16) * (D * 2) +
-                         few_piece<D>(r + 16, c) * 16 + within);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const u2 lo = transposed(mine_v + v_at[t]);
+      const u2 up = transposed(mine_v + v_at[t] + 16 * (D * 2));
       Oct<K> x;
-      x.raw = u4{lo[0], lo[1], hi[0], hi[1]};
-      return x;
-    };
-    if (seen_min < seen_max && cut && __ballot(odd_v)) {
+      x.raw = u4{lo[0], lo[1], up[0], up[1]};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const Oct<K> x = v_piece(t);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          o[rt][t] = mfma16(only<K>(x, 0).v, p[rt].v, o[rt][t]);
-          Oct<K> there;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
-            there.h[j] = (T)(key < seen[rt] ? 1.0f : 0.0f);
-          }
-          for (int kind = 1; kind < 4; ++kind) {
-            f4 hit = mfma16(only<K>(x, kind).v, there.v, f4{0, 0, 0, 0});
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              o[rt][t][j] += hit[j] > 0.0f ? special(kind) : 0.0f;
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const Oct<K> x = v_piece(t);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[rt][t] = mfma16(x.v, p[rt].v, o[rt][t]);
-      }
+      for (int rt = 0; rt < RT; ++rt)
+        o[rt][t] = mfma16(x.v, p[rt].v, o[rt][t]);
     }
     wave_fence();
   }
@@ -603,14 +632,11 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
         y[j] = none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
       __builtin_memcpy(dst + d0, y, sizeof y);
     } else {
-      float* part = a.parts + (((long long)blockIdx.x * a.splits +
-                                blockIdx.y) * BM + rt * 16 + row) * (D + 2);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) part[d0 + j] = x[j];
-      if ((threadIdx.x & 15) == 0) {
-        part[D] = top;
-        part[D + 1] = total;
-      }
+      const long long at = ((long long)blockIdx.x * a.splits + blockIdx.y) *
+                               BM + rt * 16 + row;
+      __builtin_memcpy(a.parts + at * D + d0, x, sizeof x);
+      if ((threadIdx.x & 15) == 0)
+        *reinterpret_cast<f2*>(a.stats + at * 2) = f2{top, total};
     }
   }
 }
@@ -842,9 +868,11 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
       id = page_of(kt + 2);
     }
     const int key0 = kt * BN;
-    if (key0 < wave_max) {
-      const char* kd = lds + (kt & 1) * (2 * TILE);
-      const char* vd = kd + TILE;
+    const char* kd = lds + (kt & 1) * (2 * TILE);
+    char* vd = lds + (kt & 1) * (2 * TILE) + TILE;
+    const bool works = key0 < wave_max;
+    Oct<K> p[4];
+    if (works) {
       f16v sc[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -886,7 +914,6 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
           for (int j = 0; j < 16; ++j) o[t][j] *= keep;
       }
       const float base = base_of(m);
-      Oct<K> p[4];
 #pragma unroll
       for (int j = 0; j < 32; ++j)
         p[j >> 3].h[j & 7] = (T)exp2_of(
@@ -894,47 +921,46 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         sum = add_pair(p[j >> 2], j & 3, sum);
+    }
+    if (key0 + BN > seen_min && odd_tile[kt & 1] == kt + 1) {
+      // what is not finite goes to the rows that see it, then gives way
+      if (works)
+#pragma unroll 1
+        for (int key = 0; key < BN; ++key)
+          each_strange<K, D>(
+              [&](int d) {
+                return (const T*)(vd + key * (D * 2) +
+                                  v_piece_at<D>(key, d >> 3) * 16 +
+                                  (d & 7) * 2);
+              },
+              [&](int d, float v) {
+#pragma unroll
+                for (int i = 0; i < NT * 16; ++i)
+                  if (d == (i >> 4) * 32 + (i & 3) + 8 * ((i & 15) >> 2) +
+                               4 * hi &&
+                      key0 + key < seen)
+                    o[i >> 4][i & 15] += v;
+              });
+      __syncthreads();
+#pragma unroll 1
+      for (int i = threadIdx.x; i < BN * D / 8; i += 256) {
+        Oct<K>* x = reinterpret_cast<Oct<K>*>(vd + i * 16);
+        x->raw = finite_only<K>(*x);
+      }
+      __syncthreads();
+    }
+    if (works) {
       // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
-      auto v_piece = [&](int step, int t) {
-        const char* at = vd + v_at[t] + step * 16 * (D * 2);
-        u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
-        Oct<K> x;
-        x.raw = u4{lo[0], lo[1], up[0], up[1]};
-        return x;
-      };
-      if (cut && odd_tile[kt & 1] == kt + 1) {
+#pragma unroll
+      for (int step = 0; step < 4; ++step)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          for (int kind = 1; kind < 4; ++kind) {
-            f16v hit;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) hit[j] = 0.0f;
-#pragma unroll
-            for (int step = 0; step < 4; ++step) {
-              Oct<K> there;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int key = key0 + step * 16 + (j & 3) + 8 * (j >> 2) +
-                                4 * hi;
-                there.h[j] = (T)(key < seen ? 1.0f : 0.0f);
-              }
-              hit = mfma32(only<K>(v_piece(step, t), kind).v, there.v, hit);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              o[t][j] += hit[j] > 0.0f ? special(kind) : 0.0f;
-          }
-#pragma unroll
-          for (int step = 0; step < 4; ++step)
-            o[t] = mfma32(only<K>(v_piece(step, t), 0).v, p[step].v, o[t]);
+          const char* at = vd + v_at[t] + step * 16 * (D * 2);
+          u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
+          Oct<K> x;
+          x.raw = u4{lo[0], lo[1], up[0], up[1]};
+          o[t] = mfma32(x.v, p[step].v, o[t]);
         }
-      } else {
-#pragma unroll
-        for (int step = 0; step < 4; ++step)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            o[t] = mfma32(v_piece(step, t).v, p[step].v, o[t]);
-      }
     }
     if (more) put(kt + 1);
     __syncthreads();
@@ -958,78 +984,113 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
         __builtin_memcpy(dst + t * 32 + 2 * j + 4 * hi, y, sizeof y);
       }
   } else {
-    float* part = a.parts + (((long long)(tile * a.Hk + h) * a.splits +
-                              blockIdx.y) * BM + wave * 32 + col) * (D + 2);
+    const long long at = ((long long)(tile * a.Hk + h) * a.splits +
+                          blockIdx.y) * BM + wave * 32 + col;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 16; j += 2)
-        *reinterpret_cast<f2*>(part + t * 32 + (j & 3) + 8 * (j >> 2) +
-                               4 * hi) = f2{o[t][j], o[t][j + 1]};
-    if (hi == 0) {
-      part[D] = m;
-      part[D + 1] = sum;
-    }
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<f4*>(a.parts + at * D + t * 32 + 2 * j + 4 * hi) =
+            f4{o[t][j], o[t][j + 1], o[t][j + 2], o[t][j + 3]};
+    if (hi == 0) *reinterpret_cast<f2*>(a.stats + at * 2) = f2{m, sum};
   }
 }
 
 // ---- the splits' parts ------------------------------------------------------
 
-// One workgroup for 4 rows of a tile; a wave adds up one row.
-template <typename K, int D>
+// D/4 lanes for a row's part; GS groups of them share a row's parts, and
+// are joined through LDS.
+template <typename K, int D, int GS>
 __global__ void __launch_bounds__(256)
 join_kernel(Args a, int BM, int BN, int least) {
   typedef typename K::T T;
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES, ROWS = GROUPS / GS;
+  __shared__ f4 sums[GS > 1 ? GROUPS : 1][LANES];
+  __shared__ f2 tops[GROUPS];
   const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
   const Span s = find(a, tile, BM);
   if (s.seq < 0) return;
-  const int row = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int r = s.row0 + row, lane = threadIdx.x & 63;
-  if (r >= s.rows) return;
   const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
   const Share all = share_of((seen_max + BN - 1) / BN, a.splits, 0, least);
   if (all.active == 1) return;
-  const float* part =
-      a.parts + ((long long)blockIdx.x * a.splits * BM + row) * (D + 2);
-  const long long step = (long long)BM * (D + 2);
-  float top = minus_inf();
-  for (int i = lane; i < all.active; i += 64)
-    top = fmaxf(top, part[i * step + D]);
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int row = blockIdx.y * ROWS + group / GS, r = s.row0 + row;
+  const bool real = row < BM && r < s.rows;
+  const long long at = (long long)blockIdx.x * a.splits * BM + row;
+
+  // parts group % GS, + GS, ...: 4 loads on their way at a time
+  f4 x = {0, 0, 0, 0};
+  float top = minus_inf(), total = 0.0f;
+  if (real)
+    for (int i = group % GS; i < all.active; i += 4 * GS) {
+      f4 y[4];
+      f2 st[4];
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-  const float base = base_of(top);
-  constexpr int PER = D >= 64 ? D / 64 : 1;
-  const bool works = lane * PER < D;
-  float x[PER] = {}, total = 0.0f;
-  for (int i = 0; i < all.active; ++i) {
-    const float* at = part + i * step;
-    const float keep = exp2_of(at[D] - base);
-    total += at[D + 1] * keep;
-    if (works)
+      for (int j = 0; j < 4; ++j) {
+        const int k = i + j * GS;
+        const long long from = at + (long long)min(k, all.active - 1) * BM;
+        y[j] = *reinterpret_cast<const f4*>(a.parts + from * D + lane * 4);
+        st[j] = *reinterpret_cast<const f2*>(a.stats + from * 2);
+      }
 #pragma unroll
-      for (int j = 0; j < PER; ++j) x[j] += at[lane * PER + j] * keep;
+      for (int j = 0; j < 4; ++j) {
+        if (i + j * GS >= all.active) continue;
+        const float next = fmaxf(top, st[j][0]), base = base_of(next);
+        const float old = exp2_of(top - base), now = exp2_of(st[j][0] - base);
+        x = x * old + y[j] * now;
+        total = total * old + st[j][1] * now;
+        top = next;
+      }
+    }
+  if constexpr (GS > 1) {
+    sums[group][lane] = x;
+    if (lane == 0) tops[group] = f2{top, total};
+    __syncthreads();
+    if (group % GS || !real) return;
+    float best = top;
+#pragma unroll
+    for (int g = 1; g < GS; ++g) best = fmaxf(best, tops[group + g][0]);
+    const float base = base_of(best), own = exp2_of(top - base);
+    x *= own;
+    total *= own;
+#pragma unroll
+    for (int g = 1; g < GS; ++g) {
+      const float now = exp2_of(tops[group + g][0] - base);
+      x += sums[group + g][lane] * now;
+      total += tops[group + g][1] * now;
+    }
   }
-  if (!works) return;
+  if (!real) return;
   const bool none = seen_by(a, s, r) == 0;
   const float inv = s.broken ? nan_f32() : 1.0f / total;
-  T* dst = (T*)a.out +
-           ((long long)(s.q0 + r / a.G) * a.Hq + h * a.G + r % a.G) * D;
+  T y[4];
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    dst[lane * PER + j] =
-        none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
+  for (int j = 0; j < 4; ++j)
+    y[j] = none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
+  __builtin_memcpy((T*)a.out + ((long long)(s.q0 + r / a.G) * a.Hq +
+                                h * a.G + r % a.G) * D + lane * 4,
+                   y, sizeof y);
 }
 
 // ---- launching ------------------------------------------------------------
+
+template <typename K, int D, int GS>
+int launch_join_by(Args& a, int tiles, int BM, int BN, int least,
+                   hipStream_t stream) {
+  constexpr int ROWS = 256 / (D / 4) / GS;
+  void* args[] = {&a, &BM, &BN, &least};
+  return (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&join_kernel<K, D, GS>),
+      dim3(tiles * a.Hk, (BM + ROWS - 1) / ROWS), dim3(256), args, 0, stream);
+}
 
 template <typename K, int D>
 int launch_join(Args& a, int tiles, int BM, int BN, int least,
                 hipStream_t stream) {
   if (a.splits == 1) return 0;
-  void* args[] = {&a, &BM, &BN, &least};
-  return (int)hipLaunchKernel(
-      reinterpret_cast<const void*>(&join_kernel<K, D>),
-      dim3(tiles * a.Hk, BM / 4), dim3(256), args, 0, stream);
+  return a.splits >= 16
+             ? launch_join_by<K, D, 8>(a, tiles, BM, BN, least, stream)
+             : launch_join_by<K, D, 1>(a, tiles, BM, BN, least, stream);
 }
 
 template <typename K, int D, bool Q8, int RT>
@@ -1059,11 +1120,13 @@ struct Plan {
 template <typename K, int D, bool Q8>
 int run(Args a, const Plan& p, hipStream_t stream) {
   int rc = 0;
+  float* parts = a.parts;
   if (p.few_rows) {
     a.which = p.many ? 1 : 0;
     a.splits = p.few_splits;
     const int tiles =
         p.many ? a.B : (int)((long long)a.T * a.G / p.few_rows) + a.B;
+    a.stats = parts + (long long)tiles * a.Hk * a.splits * p.few_rows * D;
     rc = p.few_rows == 16 ? launch_few<K, D, Q8, 1>(a, tiles, stream)
                           : launch_few<K, D, Q8, 2>(a, tiles, stream);
   }
@@ -1071,6 +1134,7 @@ int run(Args a, const Plan& p, hipStream_t stream) {
     a.which = p.few_rows ? 2 : 0;
     a.splits = p.many_splits;
     const int tiles = (int)((long long)a.T * a.G / 128) + a.B;
+    a.stats = parts + (long long)tiles * a.Hk * a.splits * 128 * D;
     rc = launch_many<K, D, Q8>(a, tiles, stream);
   }
   return rc;
@@ -1112,7 +1176,7 @@ int tf_paged_attention(
     return (int)hipErrorInvalidValue;
   Args a{q, k, v, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
          (const int*)q_starts, (const int*)kv_lens, (const int*)table, out,
-         (float*)parts, q_row, q_head, table_row, cols, T, B, Hq, Hk,
+         (float*)parts, nullptr, q_row, q_head, table_row, cols, T, B, Hq, Hk,
          Hq / Hk, pages, page_log2,
          // 0 times a masked score would be NaN; this leaves every p 1 too
          scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 0};
