@@ -61,10 +61,9 @@ struct Args {
   int T, B, Hq, Hk, G, pages, page_log2;
   float scale;  // times log2(e): exponentials are of base 2
   int causal, splits;
-  int which;  // 0: all sequences, 1: those of at most 32 rows, 2: the others
+  int workers;  // of the few kernel
+  int unit_log2;
 };
-
-constexpr int FEW_ROWS = 32;
 
 // ---- what is where ----------------------------------------------------
 
@@ -80,23 +79,18 @@ struct Span {
 // before it, and the last such start at or below `tile` is its sequence.
 __device__ inline Span find(const Args& a, int tile, int BM) {
   Span s;
-  int seq;
-  if (a.which == 1) {
-    seq = tile;
-  } else {
-    const int lane = threadIdx.x & 63;
-    seq = -1;
-    for (int base = 0; base < a.B; base += 64) {
-      int i = base + lane;
-      bool at = false;
-      if (i < a.B) {
-        int start = min(max(a.q_starts[i], 0), a.T);
-        at = start * a.G / BM + i <= tile;
-      }
-      int c = __popcll(__ballot(at));
-      seq += c;
-      if (c < 64) break;
+  int seq = -1;
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < a.B; base += 64) {
+    int i = base + lane;
+    bool at = false;
+    if (i < a.B) {
+      int start = min(max(a.q_starts[i], 0), a.T);
+      at = start * a.G / BM + i <= tile;
     }
+    int c = __popcll(__ballot(at));
+    seq += c;
+    if (c < 64) break;
   }
   if (seq < 0 || seq >= a.B) return s;
   int q0 = min(max(a.q_starts[seq], 0), a.T);
@@ -104,10 +98,8 @@ __device__ inline Span find(const Args& a, int tile, int BM) {
   s.n = q1 - q0;
   s.rows = s.n * a.G;
   s.q0 = q0;
-  s.row0 = a.which == 1 ? 0 : (tile - (q0 * a.G / BM + seq)) * BM;
+  s.row0 = (tile - (q0 * a.G / BM + seq)) * BM;
   if (s.row0 >= s.rows || s.row0 < 0) return s;
-  if (a.which == 1 && s.rows > FEW_ROWS) return s;
-  if (a.which == 2 && s.rows <= FEW_ROWS) return s;
   s.len = a.kv_lens[seq];
   const long long room = (long long)a.cols << a.page_log2;
   s.broken = s.len < 0 || s.len > room;
@@ -286,6 +278,211 @@ __device__ inline void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// ---- the few rows' work, in equal shares -----------------------------------
+
+// The work is one line: for each kv head, each sequence, each of its tiles of
+// rows, an item of OWN + (its keys / unit keys) units. Worker w takes the
+// units from edge(w) to edge(w + 1): w * per, moved to an item's start or end
+// where that is less than NEAR away. So workers end together however ragged
+// the batch is, items of up to 2 NEAR units are never split, and of a
+// worker's items at most two are split: one that it starts (its part is in
+// place 1), and one that it goes on with (place 0). A unit is 32 keys, or
+// more where the line would pass 2^30 units.
+constexpr int OWN = 4, NEAR = 8;
+
+struct Item {
+  int seq, tile;  // tile of the sequence's rows
+  int first;      // unit of its head's line
+  int units;
+};
+
+// 64 sequences, one a lane: the units of one of its items, and of all up to
+// its last; `before`: of the sequences before these
+struct Chunk {
+  int base, before, one, own, upto;
+};
+
+struct Line {
+  int head, per;  // units of a head's line, of a worker
+};
+
+__device__ inline Chunk chunk_of(const Args& a, int base, int before,
+                                 int BM) {
+  const int lane = threadIdx.x & 63, i = base + lane;
+  Chunk c{base, before, 0, 0, 0};
+  if (i < a.B) {
+    const int q0 = min(max(a.q_starts[i], 0), a.T);
+    const int q1 = min(max(a.q_starts[i + 1], 0), a.T);
+    const int len = a.kv_lens[i];
+    const int rows = (q1 - q0) * a.G;
+    if (rows > 0) {
+      const int unit = 32 << a.unit_log2;
+      const bool broken =
+          len < 0 || len > ((long long)a.cols << a.page_log2);
+      c.one = OWN + (broken ? 0 : (len + unit - 1) / unit);
+      c.own = (rows + BM - 1) / BM * c.one;
+    }
+  }
+  c.upto = c.own;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const int y = __shfl_up(c.upto, x, 64);
+    if (lane >= x) c.upto += y;
+  }
+  return c;
+}
+
+// the first sequences, and the line of all
+__device__ inline Line line_of(const Args& a, Chunk& c, int BM) {
+  c = chunk_of(a, 0, 0, BM);
+  Line l;
+  l.head = __builtin_amdgcn_readlane(c.upto, 63);
+  for (int base = 64; base < a.B; base += 64)
+    l.head += __builtin_amdgcn_readlane(chunk_of(a, base, 0, BM).upto, 63);
+  l.per = max((int)(((long long)l.head * a.Hk + a.workers - 1) / a.workers),
+              NEAR);
+  return l;
+}
+
+// the item of unit `at` of a head's line; at < line.head
+__device__ inline Item item_at(const Args& a, Chunk& c, int at, int BM) {
+  if (at < c.before) c = chunk_of(a, 0, 0, BM);
+  while (true) {
+    const unsigned long long over = __ballot(c.before + c.upto > at);
+    if (over) {
+      const int l = __ffsll(over) - 1;
+      Item r;
+      r.seq = c.base + l;
+      r.units = __builtin_amdgcn_readlane(c.one, l);
+      const int start = c.before + __builtin_amdgcn_readlane(c.upto, l) -
+                        __builtin_amdgcn_readlane(c.own, l);
+      r.tile = (at - start) / r.units;
+      r.first = start + r.tile * r.units;
+      return r;
+    }
+    if (c.base + 64 >= a.B) return Item{-1, 0, 0, 1};
+    c = chunk_of(a, c.base + 64,
+                 c.before + __builtin_amdgcn_readlane(c.upto, 63), BM);
+  }
+}
+
+// where worker w starts
+__device__ inline long long edge(const Args& a, const Line& l, Chunk& c,
+                                 int w, int BM) {
+  const long long at = (long long)w * l.per;
+  if (at >= (long long)l.head * a.Hk) return (long long)l.head * a.Hk;
+  const int h = (int)((uint32_t)at / (uint32_t)l.head);
+  const Item it = item_at(a, c, (int)(at - (long long)h * l.head), BM);
+  const long long first = (long long)h * l.head + it.first;
+  if (at - first < NEAR) return first;
+  return first + it.units - at < NEAR ? first + it.units : at;
+}
+
+// where the parts of an item that starts at unit `first` of the whole line
+// lie: part 0, and part i + 1 `stride` after part i from the second on
+struct Parts {
+  long long part0, part1;
+  int count, stride;
+};
+
+__device__ inline Parts parts_of(const Line& l, long long first, int units) {
+  Parts p{0, 0, 1, 2};
+  if (units < 2 * NEAR) return p;
+  // the edges inside of the item
+  const int w0 = (int)((uint32_t)(first + NEAR + l.per - 1) / (uint32_t)l.per);
+  const int w1 = (int)((uint32_t)(first + units - NEAR) / (uint32_t)l.per);
+  p.count = max(w1 - w0 + 2, 1);
+  p.part0 = 2LL * (w0 - 1) + 1;
+  p.part1 = 2LL * w0;
+  return p;
+}
+
+__device__ inline Span span_of(const Args& a, int seq, int row0) {
+  Span s;
+  s.seq = seq;
+  s.q0 = min(max(a.q_starts[seq], 0), a.T);
+  s.n = min(max(a.q_starts[seq + 1], 0), a.T) - s.q0;
+  s.rows = s.n * a.G;
+  s.row0 = row0;
+  s.len = a.kv_lens[seq];
+  s.broken = s.len < 0 || s.len > ((long long)a.cols << a.page_log2);
+  if (s.broken) s.len = 0;
+  return s;
+}
+
+// ---- the splits' parts ------------------------------------------------------
+
+// The sums of a row's parts: D/4 lanes a row (each load is of one run of
+// memory: a lane has pairs of the two halves of D); GS groups of them share a
+// row's parts, and are joined through LDS.
+template <typename K, int D, int GS>
+__device__ inline void join_rows(const Args& a, const Span& s, int h,
+                                 const Parts& p, int BM, int row0) {
+  typedef typename K::T T;
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ f4 sums[GS > 1 ? GROUPS : 1][LANES];
+  __shared__ f2 tops[GROUPS];
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int row = row0 + group / GS, r = s.row0 + row;
+  const bool real = row < BM && r < s.rows;
+
+  // parts group % GS, + GS, ...: 4 loads on their way at a time
+  f4 x = {0, 0, 0, 0};
+  float top = minus_inf(), total = 0.0f;
+  if (real)
+    for (int i = group % GS; i < p.count; i += 4 * GS) {
+      f2 y[4][2], st[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = min(i + j * GS, p.count - 1);
+        const long long from =
+            (k ? p.part1 + (long long)(k - 1) * p.stride : p.part0) * BM + row;
+        const float* at = a.parts + from * D + lane * 2;
+        y[j][0] = *reinterpret_cast<const f2*>(at);
+        y[j][1] = *reinterpret_cast<const f2*>(at + D / 2);
+        st[j] = *reinterpret_cast<const f2*>(a.stats + from * 2);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j * GS >= p.count) continue;
+        const float next = fmaxf(top, st[j][0]), base = base_of(next);
+        const float old = exp2_of(top - base), now = exp2_of(st[j][0] - base);
+        x = x * old + f4{y[j][0][0], y[j][0][1], y[j][1][0], y[j][1][1]} * now;
+        total = total * old + st[j][1] * now;
+        top = next;
+      }
+    }
+  if constexpr (GS > 1) {
+    sums[group][lane] = x;
+    if (lane == 0) tops[group] = f2{top, total};
+    __syncthreads();
+    if (group % GS || !real) return;
+    float best = top;
+#pragma unroll
+    for (int g = 1; g < GS; ++g) best = fmaxf(best, tops[group + g][0]);
+    const float base = base_of(best), own = exp2_of(top - base);
+    x *= own;
+    total *= own;
+#pragma unroll
+    for (int g = 1; g < GS; ++g) {
+      const float now = exp2_of(tops[group + g][0] - base);
+      x += sums[group + g][lane] * now;
+      total += tops[group + g][1] * now;
+    }
+  }
+  if (!real) return;
+  const bool none = seen_by(a, s, r) == 0;
+  const float inv = s.broken ? nan_f32() : 1.0f / total;
+  T* dst = (T*)a.out + ((long long)(s.q0 + r / a.G) * a.Hq + h * a.G +
+                        r % a.G) * D + lane * 2;
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const T y[2] = {none && !s.broken ? (T)0.0f : (T)(x[j] * inv),
+                    none && !s.broken ? (T)0.0f : (T)(x[j + 1] * inv)};
+    __builtin_memcpy(dst + j / 2 * (D / 2), y, sizeof y);
+  }
+}
+
 // ---- few rows ------------------------------------------------------------
 
 // Where 16-byte piece c of a wave's V row lies: the 32-byte blocks that a
@@ -297,11 +494,12 @@ __device__ inline int few_piece(int row, int c) {
   return c ^ (((row >> 2) & 1) << 1);
 }
 
-template <typename K, int D, bool Q8, int RT>
-__global__ void __launch_bounds__(256, Q8 && RT == 1 ? 3 : 2)
-few_kernel(Args a) {
+template <typename K, int D, bool Q8>
+__device__ inline void
+few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
+         const Share& mine, bool whole, long long part) {
   typedef typename K::T T;
-  constexpr int BM = 16 * RT, BN = 32, WAVES = 4;
+  constexpr int BM = 16, BN = 32, WAVES = 4;
   constexpr int NF = D / 32;              // steps of the product over D
   constexpr int NT = D / 16;              // tiles of 16 values of O^T
   constexpr int EB = Q8 ? 1 : 2;          // bytes of a cached value
@@ -312,33 +510,22 @@ few_kernel(Args a) {
   constexpr int NK = NF * 8 * EB / KB;    // K loads of a lane for 16 keys
   constexpr int JS = D + 4;               // a row of what the waves join
 
-  // V tiles while the keys pass, then the waves' sums
-  __shared__ __attribute__((aligned(16))) char
-      lds[WAVES * 16 * JS * 4 > WAVES * BN * D * 2 ? WAVES * 16 * JS * 4
-                                                   : WAVES * BN * D * 2];
-  __shared__ float stat[2][WAVES][16];
-
-  const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
-  const Span s = find(a, tile, BM);
-  if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  int lane = threadIdx.x & 63;
+  // What goes by the lane is worked out for each item anew: kept over the
+  // items it would take the registers that the tiles need.
+  asm volatile("" : "+v"(lane));
   const int col = lane & 15, grp = lane >> 4;
 
   const int seen_min = seen_by(a, s, s.row0);
   const int last_row = min(s.row0 + BM, s.rows) - 1;
   const int seen_max = seen_by(a, s, last_row);
-  const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
-                              2 * WAVES);
-  if ((int)blockIdx.y >= mine.active) return;
 
   // Q: a lane holds 8 values of row `col` for each step
-  Oct<K> q[RT][NF];
-  int seen[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = s.row0 + rt * 16 + col;
-    seen[rt] = seen_by(a, s, r);
+  Oct<K> q[NF];
+  const int seen = seen_by(a, s, s.row0 + col);
+  {
+    const int r = s.row0 + col;
     const bool real = r < s.rows;
     const int t = real ? r / a.G : 0, g = real ? r % a.G : 0;
     const T* src = (const T*)a.q + (s.q0 + t) * a.q_row +
@@ -347,11 +534,11 @@ few_kernel(Args a) {
     for (int f = 0; f < NF; ++f) {
       const int d0 = KB == 16 && Q8 ? 64 * (f >> 1) + grp * 16 + (f & 1) * 8
                                     : 32 * f + grp * 8;
-      q[rt][f].raw = real ? *reinterpret_cast<const u4*>(src + d0)
-                          : u4{0, 0, 0, 0};
+      q[f].raw = real ? *reinterpret_cast<const u4*>(src + d0)
+                      : u4{0, 0, 0, 0};
       // scores grow with the product below: a negative scale turns q
-      if (a.scale < 0.0f) q[rt][f].raw ^= u4{0x80008000u, 0x80008000u,
-                                             0x80008000u, 0x80008000u};
+      if (a.scale < 0.0f) q[f].raw ^= u4{0x80008000u, 0x80008000u,
+                                         0x80008000u, 0x80008000u};
     }
   }
   const float scale = fabsf(a.scale);
@@ -366,16 +553,18 @@ few_kernel(Args a) {
     return key < seen_max ? uniform_load(pages + (key >> a.page_log2)) : 0;
   };
 
-  u4 kr[2][NK], vr[NV];
-  uint32_t ksr[2], vsr[NV];
+  struct Arrival {
+    u4 kr[2][NK], vr[NV];
+    uint32_t ksr[2], vsr[NV];
+    bool bad0, bad1;  // halves without a page
+  };
   int id[2];  // pages of the tile to come
-  bool bad0 = false, bad1 = false;
   const uint32_t k_off = col * (D * EB) + grp * KB;
   const uint32_t v_off = lane * 16;
 
-  auto fetch = [&](int kt) {
-    bad0 = (unsigned)id[0] >= (unsigned)a.pages;
-    bad1 = (unsigned)id[1] >= (unsigned)a.pages;
+  auto fetch = [&](Arrival& to, int kt) {
+    const bool bad0 = to.bad0 = (unsigned)id[0] >= (unsigned)a.pages;
+    const bool bad1 = to.bad1 = (unsigned)id[1] >= (unsigned)a.pages;
     const int key = kt * BN;
     const long long row0 = (((long long)(bad0 ? 0 : id[0]) * a.Hk + h)
                             << a.page_log2) + (key & in_page);
@@ -385,14 +574,14 @@ few_kernel(Args a) {
     for (int half = 0; half < 2; ++half) {
       const long long row = half ? row1 : row0;
       const uint8_t* src = kc + row * (D * EB);
-      if constexpr (Q8) ksr[half] = (a.k_scale + row)[col];
+      if constexpr (Q8) to.ksr[half] = (a.k_scale + row)[col];
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         if constexpr (KB == 16) {
-          kr[half][i] = *reinterpret_cast<const u4*>(src + k_off + i * 64);
+          to.kr[half][i] = *reinterpret_cast<const u4*>(src + k_off + i * 64);
         } else {
           u2 x = *reinterpret_cast<const u2*>(src + k_off);
-          kr[half][i] = u4{x[0], x[1], 0, 0};
+          to.kr[half][i] = u4{x[0], x[1], 0, 0};
         }
       }
     }
@@ -402,27 +591,22 @@ few_kernel(Args a) {
         constexpr int PER16 = 16 / (VROWS > 16 ? 16 : VROWS);
         const long long row =
             (i / PER16 ? row1 : row0) + (i % PER16) * VROWS;
-        if constexpr (Q8) vsr[i] = (a.v_scale + row)[lane / LPR];
-        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) + v_off);
+        if constexpr (Q8) to.vsr[i] = (a.v_scale + row)[lane / LPR];
+        to.vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) + v_off);
       } else {  // one load takes both halves
         const int vrow = lane / LPR;
         const long long row = (vrow < 16 ? row0 : row1) + (vrow & 15);
-        if constexpr (Q8) vsr[i] = a.v_scale[row];
-        vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
+        if constexpr (Q8) to.vsr[i] = a.v_scale[row];
+        to.vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
                                              (lane % LPR) * 16);
       }
     }
   };
 
-  f4 o[RT][NT];
-  float m[RT], sum[RT];
+  f4 o[NT];
+  float m = minus_inf(), sum = 0.0f;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = minus_inf();
-    sum[rt] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[rt][t] = f4{0, 0, 0, 0};
-  }
+  for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
 
   char* mine_v = lds + wave * (BN * D * 2);
   uint32_t v_at[NT];  // a lane's 4 keys by 4 values of transposing reads
@@ -434,39 +618,47 @@ few_kernel(Args a) {
                 few_piece<D>(row, t * 2 + ((col >> 1) & 1)) * 16 +
                 (col & 1) * 8;
   }
+  // 8-bit tiles: two on their way in turn, since widening one takes long
+  constexpr int AHEAD = Q8 ? 1 : 0;
+  Arrival arrivals[1 + AHEAD];
   int kt = mine.first + wave;
   if (kt < mine.last) {
     id[0] = page_of(kt * BN);
     id[1] = page_of(kt * BN + 16);
-    fetch(kt);
+    fetch(arrivals[0], kt);
     id[0] = page_of((kt + WAVES) * BN);
     id[1] = page_of((kt + WAVES) * BN + 16);
   }
-  for (; kt < mine.last; kt += WAVES) {
+  auto fetch_next = [&](Arrival& to) {
+    if (kt + WAVES < mine.last) {
+      fetch(to, kt + WAVES);
+      id[0] = page_of((kt + 2 * WAVES) * BN);
+      id[1] = page_of((kt + 2 * WAVES) * BN + 16);
+    }
+  };
+  auto take = [&](Arrival& now, Arrival& next) {
+    if constexpr (AHEAD) fetch_next(next);
     const int key0 = kt * BN;
-    const bool none0 = bad0, none1 = bad1;  // halves without a page
+    const bool none0 = now.bad0, none1 = now.bad1;
 
     // S^T: 2 tiles of 16 keys
-    f4 sc[RT][2];
+    f4 sc[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[rt][half] = f4{0, 0, 0, 0};
+      sc[half] = f4{0, 0, 0, 0};
       float scale = 1.0f;
-      if constexpr (Q8) scale = scale_of(ksr[half]);
+      if constexpr (Q8) scale = scale_of(now.ksr[half]);
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         Oct<K> x;
         if constexpr (Q8) {
-          const u4 w = kr[half][KB == 16 ? f >> 1 : f];
+          const u4 w = now.kr[half][KB == 16 ? f >> 1 : f];
           widen(x, (KB == 16 && (f & 1)) ? u2{w[2], w[3]} : u2{w[0], w[1]},
                 scale);
         } else {
-          x.raw = kr[half][f];
+          x.raw = now.kr[half][f];
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          sc[rt][half] = mfma16(x.v, q[rt][f].v, sc[rt][half]);
+        sc[half] = mfma16(x.v, q[f].v, sc[half]);
       }
     }
 
@@ -480,15 +672,15 @@ few_kernel(Args a) {
       const int vrow = i * VROWS + lane / LPR;
       if (past) {
         if (key0 + vrow >= seen_max || (vrow < 16 ? none0 : none1)) {
-          vr[i] = u4{0, 0, 0, 0};
-          vsr[i] = 127;
+          now.vr[i] = u4{0, 0, 0, 0};
+          now.vsr[i] = 127;
         }
       }
       if constexpr (Q8) {
-        const float scale = scale_of(vsr[i]);
+        const float scale = scale_of(now.vsr[i]);
         Oct<K> x, y;
-        widen(x, u2{vr[i][0], vr[i][1]}, scale);
-        widen(y, u2{vr[i][2], vr[i][3]}, scale);
+        widen(x, u2{now.vr[i][0], now.vr[i][1]}, scale);
+        widen(y, u2{now.vr[i][2], now.vr[i][3]}, scale);
         if (look) odd_v |= strange(x) || strange(y);
         const int c = (lane % LPR) * 2;
         char* row = mine_v + vrow * (D * 2);
@@ -496,7 +688,7 @@ few_kernel(Args a) {
         *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c + 1) * 16) = y.raw;
       } else {
         Oct<K> x;
-        x.raw = vr[i];
+        x.raw = now.vr[i];
         if (look) odd_v |= strange(x);
         *reinterpret_cast<u4*>(mine_v + vrow * (D * 2) +
                                few_piece<D>(vrow, lane % LPR) * 16) = x.raw;
@@ -505,44 +697,37 @@ few_kernel(Args a) {
     wave_fence();
 
     // the next tile is on its way while this one's softmax is worked out
-    if (kt + WAVES < mine.last) {
-      fetch(kt + WAVES);
-      id[0] = page_of((kt + 2 * WAVES) * BN);
-      id[1] = page_of((kt + 2 * WAVES) * BN + 16);
-    }
+    if constexpr (!AHEAD) fetch_next(next);
 
-    Oct<K> p[RT];
+    Oct<K> p;
+    if (cut) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (cut) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
-          if ((j >> 2) ? none1 : none0) sc[rt][j >> 2][j & 3] = nan_f32();
-          if (key >= seen[rt]) sc[rt][j >> 2][j & 3] = minus_inf();
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int key = key0 + (j >> 2) * 16 + grp * 4 + (j & 3);
+        if ((j >> 2) ? none1 : none0) sc[j >> 2][j & 3] = nan_f32();
+        if (key >= seen) sc[j >> 2][j & 3] = minus_inf();
       }
-      float top = sc[rt][0][0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[rt][j >> 2][j & 3]);
-      top = lane_xor32_max(lane_xor16_max(top)) * scale;
-      // as in the other kernel, the maximum moves by steps of 2^8 or more
-      if (__ballot(top > m[rt] + 8.0f)) {
-        const float next = fmaxf(m[rt], top);
-        const float keep = exp2_of(m[rt] - base_of(next));
-        m[rt] = next;
-        sum[rt] *= keep;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[rt][t] *= keep;
-      }
-      const float base = base_of(m[rt]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        p[rt].h[j] = (T)exp2_of(
-            __builtin_fmaf(sc[rt][j >> 2][j & 3], scale, -base));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum[rt] = add_pair(p[rt], j, sum[rt]);
     }
+    float top = sc[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
+    top = lane_xor32_max(lane_xor16_max(top)) * scale;
+    // as in the other kernel, the maximum moves by steps of 2^8 or more
+    if (__ballot(top > m + 8.0f)) {
+      const float next = fmaxf(m, top);
+      const float keep = exp2_of(m - base_of(next));
+      m = next;
+      sum *= keep;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t] *= keep;
+    }
+    const float base = base_of(m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      p.h[j] = (T)exp2_of(
+          __builtin_fmaf(sc[j >> 2][j & 3], scale, -base));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = add_pair(p, j, sum);
 
     if (look && __ballot(odd_v)) {
       // what is not finite goes to the rows that see it, then gives way
@@ -555,12 +740,10 @@ few_kernel(Args a) {
             },
             [&](int d, float v) {
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int i = 0; i < NT * 4; ++i)
-                  if (d == (i >> 2) * 16 + grp * 4 + (i & 3) &&
-                      key0 + key < seen[rt])
-                    o[rt][i >> 2][i & 3] += v;
+              for (int i = 0; i < NT * 4; ++i)
+                if (d == (i >> 2) * 16 + grp * 4 + (i & 3) &&
+                    key0 + key < seen)
+                  o[i >> 2][i & 3] += v;
             });
       wave_fence();
 #pragma unroll 1
@@ -579,65 +762,109 @@ few_kernel(Args a) {
       const u2 up = transposed(mine_v + v_at[t] + 16 * (D * 2));
       Oct<K> x;
       x.raw = u4{lo[0], lo[1], up[0], up[1]};
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        o[rt][t] = mfma16(x.v, p[rt].v, o[rt][t]);
+      o[t] = mfma16(x.v, p.v, o[t]);
     }
     wave_fence();
+  };
+  while (kt < mine.last) {
+    take(arrivals[0], arrivals[AHEAD]);
+    kt += WAVES;
+    if constexpr (AHEAD) {
+      if (kt >= mine.last) break;
+      take(arrivals[1], arrivals[0]);
+      kt += WAVES;
+    }
   }
 
-  // join the waves, 16 rows at a time
+  // join the waves
   float(*all)[16][JS] = reinterpret_cast<float(*)[16][JS]>(lds);
+  __syncthreads();
+  const float l = lane_xor32_add(lane_xor16_add(sum));
+  if (grp == 0) {
+    stat[0][wave][col] = m;
+    stat[1][wave][col] = l;
+  }
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    __syncthreads();
-    const float l = lane_xor32_add(lane_xor16_add(sum[rt]));
-    if (grp == 0) {
-      stat[0][wave][col] = m[rt];
-      stat[1][wave][col] = l;
-    }
+  for (int t = 0; t < NT; ++t)
+    *reinterpret_cast<f4*>(&all[wave][col][t * 16 + grp * 4]) = o[t];
+  __syncthreads();
+  const int row = threadIdx.x >> 4, r = s.row0 + row;
+  if (r >= s.rows) return;
+  float top = minus_inf();
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      *reinterpret_cast<f4*>(&all[wave][col][t * 16 + grp * 4]) = o[rt][t];
-    __syncthreads();
-    const int row = threadIdx.x >> 4, r = s.row0 + rt * 16 + row;
-    if (r >= s.rows) continue;
-    float top = minus_inf();
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[0][w][row]);
+  const float base = base_of(top);
+  float keep[WAVES], total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[0][w][row]);
-    const float base = base_of(top);
-    float keep[WAVES], total = 0.0f;
+  for (int w = 0; w < WAVES; ++w) {
+    keep[w] = exp2_of(stat[0][w][row] - base);
+    total += stat[1][w][row] * keep[w];
+  }
+  // pairs of values, 16 lanes a row: stores of one run of memory
+  const int d0 = (threadIdx.x & 15) * 2;
+  const int t = r / a.G, g = r % a.G;
+  const bool none = seen_by(a, s, r) == 0;
+  const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
+  T* dst = (T*)a.out + ((long long)(s.q0 + t) * a.Hq + h * a.G + g) * D;
+  const long long at = part * BM + row;
+#pragma unroll
+  for (int d = d0; d < D; d += 32) {
+    float x = 0.0f, y = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      keep[w] = exp2_of(stat[0][w][row] - base);
-      total += stat[1][w][row] * keep[w];
+      const f2 v = *reinterpret_cast<const f2*>(&all[w][row][d]);
+      x += v[0] * keep[w];
+      y += v[1] * keep[w];
     }
-    constexpr int PER = D / 16;
-    const int d0 = (threadIdx.x & 15) * PER;
-    float x[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      x[j] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) x[j] += all[w][row][d0 + j] * keep[w];
-    }
-    if (mine.active == 1) {
-      const int t = r / a.G, g = r % a.G;
-      const bool none = seen_by(a, s, r) == 0;
-      const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
-      T* dst = (T*)a.out + ((long long)(s.q0 + t) * a.Hq + h * a.G + g) * D;
-      T y[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        y[j] = none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
-      __builtin_memcpy(dst + d0, y, sizeof y);
+    if (whole) {
+      const T z[2] = {none && !s.broken ? (T)0.0f : (T)(x * inv),
+                      none && !s.broken ? (T)0.0f : (T)(y * inv)};
+      __builtin_memcpy(dst + d, z, sizeof z);
     } else {
-      const long long at = ((long long)blockIdx.x * a.splits + blockIdx.y) *
-                               BM + rt * 16 + row;
-      __builtin_memcpy(a.parts + at * D + d0, x, sizeof x);
-      if ((threadIdx.x & 15) == 0)
-        *reinterpret_cast<f2*>(a.stats + at * 2) = f2{top, total};
+      *reinterpret_cast<f2*>(a.parts + at * D + d) = f2{x, y};
     }
+  }
+  if (!whole && d0 == 0)
+    *reinterpret_cast<f2*>(a.stats + at * 2) = f2{top, total};
+}
+
+template <typename K, int D, bool Q8>
+__global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
+  constexpr int BM = 16, BN = 32, WAVES = 4;
+  constexpr int JOIN = WAVES * 16 * (D + 4) * 4, TILES = WAVES * BN * D * 2;
+  // V tiles while the keys pass, then the waves' sums
+  __shared__ __attribute__((aligned(16))) char
+      lds[JOIN > TILES ? JOIN : TILES];
+  __shared__ float stat[2][WAVES][16];
+
+  Chunk c;
+  const Line line = line_of(a, c, BM);
+  if (line.head == 0) return;
+  // neighbouring shares go to one XCD: they read the same sequence
+  const int w = a.workers % 8 ? blockIdx.x
+                              : blockIdx.x % 8 * (a.workers / 8) +
+                                    blockIdx.x / 8;
+  long long at = edge(a, line, c, w, BM);
+  const long long end = edge(a, line, c, w + 1, BM);
+  while (at < end) {
+    const int h = (int)((uint32_t)at / (uint32_t)line.head);
+    const long long start = (long long)h * line.head;
+    const Item it = item_at(a, c, (int)(at - start), BM);
+    if (it.seq < 0) return;
+    const Span s = span_of(a, it.seq, it.tile * BM);
+    const int from = (int)(at - start) - it.first;
+    const int to = (int)min((long long)it.units, from + (end - at));
+    // an item's last units may hold no key that its rows see
+    const int all =
+        (seen_by(a, s, min(s.row0 + BM, s.rows) - 1) + BN - 1) / BN;
+    Share mine;
+    mine.first = min(max(from - OWN, 0) << a.unit_log2, all);
+    mine.last = min(max(to - OWN, 0) << a.unit_log2, all);
+    const bool whole = from == 0 && to == it.units;
+    few_part<K, D, Q8>(a, lds, stat, s, h, mine, whole,
+                           2LL * w + (from == 0 ? 1 : 0));
+    at += to - from;
+    __syncthreads();
   }
 }
 
@@ -996,80 +1223,38 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   }
 }
 
-// ---- the splits' parts ------------------------------------------------------
-
-// D/4 lanes for a row's part; GS groups of them share a row's parts, and
-// are joined through LDS.
+// One workgroup for ROWS rows of a tile.
+// BN, least: what the many kernel shared its keys by; 0: the parts of the
+// few kernel.
 template <typename K, int D, int GS>
 __global__ void __launch_bounds__(256)
 join_kernel(Args a, int BM, int BN, int least) {
-  typedef typename K::T T;
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES, ROWS = GROUPS / GS;
-  __shared__ f4 sums[GS > 1 ? GROUPS : 1][LANES];
-  __shared__ f2 tops[GROUPS];
+  constexpr int ROWS = 256 / (D / 4) / GS;
   const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
   const Span s = find(a, tile, BM);
   if (s.seq < 0) return;
-  const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
-  const Share all = share_of((seen_max + BN - 1) / BN, a.splits, 0, least);
-  if (all.active == 1) return;
-  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  const int row = blockIdx.y * ROWS + group / GS, r = s.row0 + row;
-  const bool real = row < BM && r < s.rows;
-  const long long at = (long long)blockIdx.x * a.splits * BM + row;
-
-  // parts group % GS, + GS, ...: 4 loads on their way at a time
-  f4 x = {0, 0, 0, 0};
-  float top = minus_inf(), total = 0.0f;
-  if (real)
-    for (int i = group % GS; i < all.active; i += 4 * GS) {
-      f4 y[4];
-      f2 st[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = i + j * GS;
-        const long long from = at + (long long)min(k, all.active - 1) * BM;
-        y[j] = *reinterpret_cast<const f4*>(a.parts + from * D + lane * 4);
-        st[j] = *reinterpret_cast<const f2*>(a.stats + from * 2);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j * GS >= all.active) continue;
-        const float next = fmaxf(top, st[j][0]), base = base_of(next);
-        const float old = exp2_of(top - base), now = exp2_of(st[j][0] - base);
-        x = x * old + y[j] * now;
-        total = total * old + st[j][1] * now;
-        top = next;
-      }
-    }
-  if constexpr (GS > 1) {
-    sums[group][lane] = x;
-    if (lane == 0) tops[group] = f2{top, total};
-    __syncthreads();
-    if (group % GS || !real) return;
-    float best = top;
-#pragma unroll
-    for (int g = 1; g < GS; ++g) best = fmaxf(best, tops[group + g][0]);
-    const float base = base_of(best), own = exp2_of(top - base);
-    x *= own;
-    total *= own;
-#pragma unroll
-    for (int g = 1; g < GS; ++g) {
-      const float now = exp2_of(tops[group + g][0] - base);
-      x += sums[group + g][lane] * now;
-      total += tops[group + g][1] * now;
-    }
+  Parts p;
+  if (BN) {
+    const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
+    p.count = share_of((seen_max + BN - 1) / BN, a.splits, 0, least).active;
+    p.part0 = (long long)blockIdx.x * a.splits;
+    p.part1 = p.part0 + 1;
+    p.stride = 1;
+  } else {
+    Chunk c;
+    const Line line = line_of(a, c, BM);
+    while (c.base + 64 <= s.seq)
+      c = chunk_of(a, c.base + 64,
+                   c.before + __builtin_amdgcn_readlane(c.upto, 63), BM);
+    const int l = s.seq - c.base;
+    const int units = __builtin_amdgcn_readlane(c.one, l);
+    p = parts_of(line, (long long)h * line.head + c.before +
+                           __builtin_amdgcn_readlane(c.upto, l) -
+                           __builtin_amdgcn_readlane(c.own, l) +
+                           s.row0 / BM * units, units);
   }
-  if (!real) return;
-  const bool none = seen_by(a, s, r) == 0;
-  const float inv = s.broken ? nan_f32() : 1.0f / total;
-  T y[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    y[j] = none && !s.broken ? (T)0.0f : (T)(x[j] * inv);
-  __builtin_memcpy((T*)a.out + ((long long)(s.q0 + r / a.G) * a.Hq +
-                                h * a.G + r % a.G) * D + lane * 4,
-                   y, sizeof y);
+  if (p.count == 1) return;
+  join_rows<K, D, GS>(a, s, h, p, BM, blockIdx.y * ROWS);
 }
 
 // ---- launching ------------------------------------------------------------
@@ -1087,57 +1272,39 @@ int launch_join_by(Args& a, int tiles, int BM, int BN, int least,
 template <typename K, int D>
 int launch_join(Args& a, int tiles, int BM, int BN, int least,
                 hipStream_t stream) {
-  if (a.splits == 1) return 0;
-  return a.splits >= 16
+  const int parts = BN ? a.splits : a.workers / (tiles * a.Hk);
+  return parts >= 16
              ? launch_join_by<K, D, 8>(a, tiles, BM, BN, least, stream)
              : launch_join_by<K, D, 1>(a, tiles, BM, BN, least, stream);
 }
 
-template <typename K, int D, bool Q8, int RT>
-int launch_few(Args& a, int tiles, hipStream_t stream) {
-  void* args[] = {&a};
-  int rc = (int)hipLaunchKernel(
-      reinterpret_cast<const void*>(&few_kernel<K, D, Q8, RT>),
-      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
-  return rc ? rc : launch_join<K, D>(a, tiles, 16 * RT, 32, 8, stream);
-}
-
-template <typename K, int D, bool Q8>
-int launch_many(Args& a, int tiles, hipStream_t stream) {
-  void* args[] = {&a, &tiles};
-  int rc = (int)hipLaunchKernel(
-      reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
-      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
-  return rc ? rc : launch_join<K, D>(a, tiles, 128, 64, 4, stream);
-}
-
-// rows of a tile of the few kernel: 16, 32, or 0 for none; the same for
-// many: whether it runs. Both run where the batch may hold either kind.
+// workers: of the few kernel, 0 where the many kernel runs; join: whether a
+// sequence may be long enough for it to be split; splits: of the many kernel.
 struct Plan {
-  int few_rows, few_splits, many, many_splits;
+  int workers, join, splits;
 };
 
 template <typename K, int D, bool Q8>
 int run(Args a, const Plan& p, hipStream_t stream) {
-  int rc = 0;
-  float* parts = a.parts;
-  if (p.few_rows) {
-    a.which = p.many ? 1 : 0;
-    a.splits = p.few_splits;
-    const int tiles =
-        p.many ? a.B : (int)((long long)a.T * a.G / p.few_rows) + a.B;
-    a.stats = parts + (long long)tiles * a.Hk * a.splits * p.few_rows * D;
-    rc = p.few_rows == 16 ? launch_few<K, D, Q8, 1>(a, tiles, stream)
-                          : launch_few<K, D, Q8, 2>(a, tiles, stream);
+  const int BM = p.workers ? 16 : 128;
+  int tiles = (int)((long long)a.T * a.G / BM) + a.B;
+  if (p.workers) {
+    a.workers = p.workers;
+    a.stats = a.parts + 2LL * a.workers * BM * D;
+    void* args[] = {&a};
+    int rc = (int)hipLaunchKernel(
+        reinterpret_cast<const void*>(&few_kernel<K, D, Q8>),
+        dim3(a.workers), dim3(256), args, 0, stream);
+    return rc || !p.join ? rc : launch_join<K, D>(a, tiles, BM, 0, 0, stream);
   }
-  if (!rc && p.many) {
-    a.which = p.few_rows ? 2 : 0;
-    a.splits = p.many_splits;
-    const int tiles = (int)((long long)a.T * a.G / 128) + a.B;
-    a.stats = parts + (long long)tiles * a.Hk * a.splits * 128 * D;
-    rc = launch_many<K, D, Q8>(a, tiles, stream);
-  }
-  return rc;
+  a.splits = p.splits;
+  a.stats = a.parts + (long long)tiles * a.Hk * a.splits * BM * D;
+  void* args[] = {&a, &tiles};
+  int rc = (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
+      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
+  return rc || a.splits == 1 ? rc
+                             : launch_join<K, D>(a, tiles, BM, 64, 4, stream);
 }
 
 template <typename K, bool Q8>
@@ -1154,23 +1321,22 @@ int run_d(const Args& a, const Plan& p, int D, hipStream_t stream) {
 
 extern "C" {
 
-// parts: 32-bit floats, for each kernel that splits tiles * Hk * splits *
-// rows of a tile * (D + 2) of them; the two kernels use the same ones, one
-// after the other.
+// parts: 32-bit floats, 2 * workers * 16 * (D + 2) of them where the few
+// kernel's items may be split, tiles * Hk * splits * 128 * (D + 2) for the
+// many kernel's splits.
 int tf_paged_attention(
     const void* q, const void* k, const void* v, const void* k_scale,
     const void* v_scale, const void* q_starts, const void* kv_lens,
     const void* table, void* out, void* parts, long long q_row,
     long long q_head, long long table_row, int cols, int T, int B, int Hq,
     int Hk, int pages, int page_log2, int D, float scale, int causal,
-    int fp16, int few_rows, int few_splits, int many, int many_splits,
+    int fp16, int workers, int join, int splits,
     void* stream) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || cols < 0 ||
       pages < 1 || page_log2 < 4 || page_log2 > 10 ||
-      (few_rows != 0 && few_rows != 16 && few_rows != 32) ||
-      (many && few_rows == 16) || (!many && !few_rows) || few_splits < 1 ||
-      few_splits > 65535 || many_splits < 1 || many_splits > 65535 ||
-      ((few_splits > 1 || many_splits > 1) && !parts) ||
+      workers < 0 || splits < 1 || splits > 65535 ||
+      (workers && !join && (cols << page_log2) > (2 * NEAR - OWN) * 32) ||
+      ((join || splits > 1) && !parts) ||
       ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
       (long long)T * (Hq / Hk) >= (1LL << 31))
     return (int)hipErrorInvalidValue;
@@ -1179,8 +1345,14 @@ int tf_paged_attention(
          (float*)parts, nullptr, q_row, q_head, table_row, cols, T, B, Hq, Hk,
          Hq / Hk, pages, page_log2,
          // 0 times a masked score would be NaN; this leaves every p 1 too
-         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 0};
-  const Plan p{few_rows, few_splits, many, many_splits};
+         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 1, 0};
+  // a line of less than 2^30 units, as bounded by what the host knows
+  const double items = ((double)T * (Hq / Hk) / 16 + B) * Hk;
+  while (items * (OWN + ((double)cols * (1 << page_log2) /
+                         (32 << a.unit_log2)) + 1) >= (double)(1 << 30) &&
+         a.unit_log2 < 25)
+    ++a.unit_log2;
+  const Plan p{workers, join, splits};
   const bool q8 = k_scale != nullptr;
   hipStream_t st = (hipStream_t)stream;
   return fp16 ? (q8 ? run_d<Fp16, true>(a, p, D, st)

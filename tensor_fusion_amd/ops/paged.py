@@ -116,7 +116,7 @@ _ENTRIES = {
                       + [_L] + [_I] * 6 + [_P],
     "tf_paged_read": [_P] * 4 + [_L, _I] + [_P] * 3 + [_I] * 4 + [_P],
     "tf_paged_attention": [_P] * 10 + [_L] * 3 + [_I] * 8
-                          + [ctypes.c_float] + [_I] * 6 + [_P],
+                          + [ctypes.c_float] + [_I] * 5 + [_P],
 }
 _READY = {}
 
@@ -289,29 +289,20 @@ def kv_read(cache: PagedKVCache, slots, dtype=None):
 
 
 def _plan(T: int, B: int, G: int, Hk: int, keys: int):
-    """Which kernels run, and over how many splits of the keys: (few_rows,
-    few_splits, many, many_splits). What a batch holds lies on the device;
-    this goes by its mean, and is right for any batch. A sequence of at most
-    32 rows (new tokens * G) is work for the kernel for few rows; where both
-    kinds may be there, both kernels run, each over its own sequences."""
+    """(workers, join, splits). What a batch holds lies on the device; this
+    goes by its mean, and is right for any batch. Up to 16 rows (new tokens
+    * G) a sequence are work for the kernel for few rows, whose `workers`
+    share it out among themselves; 0 workers: the kernel for many rows, with
+    the keys of each tile of 128 rows in `splits` parts."""
 
     rows = T * G
-    few_rows = many = 0
-    if rows <= 16 * B:
-        few_rows = 16
-    elif B == 1 or T == B:  # one sequence, or (most likely) one token each
-        few_rows, many = (32, 0) if rows <= 32 * B else (0, 1)
-    else:
-        few_rows, many = 32, 1
     pieces = max(1, -(-keys // 256))  # of keys that are worth a workgroup
-    few_splits = many_splits = 1
-    if few_rows:
-        busy = Hk * (B if many else max(B, rows // few_rows))
-        few_splits = min(pieces, max(1, 1024 // busy))
-    if many:
-        busy = Hk * max(B, rows // 128)
-        many_splits = min(pieces, max(1, 512 // busy))
-    return few_rows, few_splits, many, many_splits
+    if rows <= 16 * B:
+        # two workgroups fit a unit; neighbouring ones share an XCD of eight
+        items = Hk * max(B, rows // 16)
+        workers = -(-min(512, items * pieces) // 8) * 8
+        return workers, int(keys > 384), 1  # 384: never split
+    return 0, 0, min(pieces, max(1, 512 // (Hk * max(B, rows // 128))))
 
 
 def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
@@ -377,18 +368,13 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
     if T == 0 or B == 0:
         return out
     q = _rows(q)
-    few_rows, few_splits, many, many_splits = _plan(
-        T, B, G, Hk, cols * cache.page_size)
-    need = 0
-    if few_splits > 1:
-        tiles = B if many else T * G // few_rows + B
-        need = tiles * few_splits * few_rows
-    if many_splits > 1:
-        need = max(need, (T * G // 128 + B) * many_splits * 128)
+    workers, join, splits = _plan(T, B, G, Hk, cols * cache.page_size)
     parts = None
-    if need:
+    if join or splits > 1:
         # its own for every call: two captured graphs never share it
-        parts = torch.empty(need * Hk * (D + 2), dtype=torch.float32,
+        rows = 2 * workers * 16 if workers else \
+            (T * G // 128 + B) * Hk * splits * 128
+        parts = torch.empty(rows * (D + 2), dtype=torch.float32,
                             device=q.device)
     kp, vp, ks, vs = cache._ptrs
     _launch("tf_paged_attention", cache.device, q.data_ptr(), kp, vp, ks, vs,
@@ -396,6 +382,5 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
             out.data_ptr(), None if parts is None else parts.data_ptr(),
             q.stride(0), q.stride(1), block_table.stride(0), cols, T, B, Hq,
             Hk, cache.pages, cache.page_log2, D, scale, causal,
-            q.dtype is torch.float16, few_rows, few_splits, many,
-            many_splits)
+            q.dtype is torch.float16, workers, join, splits)
     return out

@@ -377,6 +377,21 @@ def test_attention_past_32_bits():
     assert torch.equal(a, k) and torch.equal(b, -k)
 
 
+@pytest.mark.parametrize("most", [3, 200], ids=["few", "many"])
+@pytest.mark.parametrize("count", [65, 300])
+def test_attention_many_sequences(count, most):
+    """More sequences than a wave has lanes, empty ones among them."""
+
+    g = torch.Generator().manual_seed(count)
+    new = torch.randint(0, 4, (count,), generator=g)
+    new[5], new[-2] = most, most
+    past = torch.randint(0, 60, (count,), generator=g)
+    past[7] = 3000
+    seqs = [(int(n), int(n + p)) for n, p in zip(new, past)]
+    b = Batch(seqs, 4, 2, 32, 64, BF16, False, seed=count, extra_cols=0)
+    check(b.run(), *b.want())
+
+
 @KEPT
 def test_attention_a_very_long_sequence(quantized):
     b = Batch([(2, 40000)], 4, 1, 64, 64, BF16, quantized, seed=15)

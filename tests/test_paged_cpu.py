@@ -147,23 +147,21 @@ def test_attention_refusals():
                                    (613, 9, 1), (60, 12, 4), (33, 1, 1),
                                    (5000, 300, 7), (2, 2, 128)])
 def test_plan_covers_every_row(T, B, G):
-    """Whatever the lengths, each sequence's tiles fit the grid, and each
-    sequence belongs to one kernel."""
+    """Whatever the lengths, each sequence's tiles fit the grid."""
 
-    few_rows, few_splits, many, many_splits = paged._plan(T, B, G, 8, 4096)
-    assert few_rows or many
-    assert not (many and few_rows == 16)
-    assert 1 <= few_splits <= 16 and 1 <= many_splits <= 16
-    if not (few_rows and many):
-        BM = 128 if many else few_rows
-        tiles = T * G // BM + B
-        gen = torch.Generator().manual_seed(T)
-        for _ in range(20):
-            cuts = torch.randint(0, T + 1, (B - 1,), generator=gen).sort()[0]
-            starts = [0, *cuts.tolist(), T]
-            end = 0
-            for i in range(B):
-                first = starts[i] * G // BM + i
-                assert first >= end
-                end = first + -(-(starts[i + 1] - starts[i]) * G // BM)
-            assert end <= tiles
+    workers, join, splits = paged._plan(T, B, G, 8, 4096)
+    assert 1 <= splits <= 16
+    assert workers == 0 or (join and 8 <= workers <= 512
+                            and workers % 8 == 0)
+    BM = 16 if workers else 128
+    tiles = T * G // BM + B
+    gen = torch.Generator().manual_seed(T)
+    for _ in range(20):
+        cuts = torch.randint(0, T + 1, (B - 1,), generator=gen).sort()[0]
+        starts = [0, *cuts.tolist(), T]
+        end = 0
+        for i in range(B):
+            first = starts[i] * G // BM + i
+            assert first >= end
+            end = first + -(-(starts[i + 1] - starts[i]) * G // BM)
+        assert end <= tiles
