@@ -74,40 +74,6 @@ struct Span {
   bool broken;     // a length that the table cannot hold
 };
 
-// Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
-// leaves each at least its own number, needs no sum over the sequences
-// before it, and the last such start at or below `tile` is its sequence.
-__device__ inline Span find(const Args& a, int tile, int BM) {
-  Span s;
-  int seq = -1;
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < a.B; base += 64) {
-    int i = base + lane;
-    bool at = false;
-    if (i < a.B) {
-      int start = min(max(a.q_starts[i], 0), a.T);
-      at = start * a.G / BM + i <= tile;
-    }
-    int c = __popcll(__ballot(at));
-    seq += c;
-    if (c < 64) break;
-  }
-  if (seq < 0 || seq >= a.B) return s;
-  int q0 = min(max(a.q_starts[seq], 0), a.T);
-  int q1 = min(max(a.q_starts[seq + 1], 0), a.T);
-  s.n = q1 - q0;
-  s.rows = s.n * a.G;
-  s.q0 = q0;
-  s.row0 = (tile - (q0 * a.G / BM + seq)) * BM;
-  if (s.row0 >= s.rows || s.row0 < 0) return s;
-  s.len = a.kv_lens[seq];
-  const long long room = (long long)a.cols << a.page_log2;
-  s.broken = s.len < 0 || s.len > room;
-  if (s.broken) s.len = 0;
-  s.seq = seq;
-  return s;
-}
-
 // how many of the sequence's keys row r sees
 __device__ inline int seen_by(const Args& a, const Span& s, int r) {
   if (r >= s.rows) return 0;
@@ -296,10 +262,11 @@ struct Item {
   int units;
 };
 
-// 64 sequences, one a lane: the units of one of its items, and of all up to
-// its last; `before`: of the sequences before these
+// 64 sequences, one a lane: its tokens and keys (-1: a length that the table
+// cannot hold), the units of one of its items, and of all up to its last;
+// `before`: of the sequences before these
 struct Chunk {
-  int base, before, one, own, upto;
+  int base, before, q0, n, len, one, own, upto;
 };
 
 struct Line {
@@ -309,18 +276,17 @@ struct Line {
 __device__ inline Chunk chunk_of(const Args& a, int base, int before,
                                  int BM) {
   const int lane = threadIdx.x & 63, i = base + lane;
-  Chunk c{base, before, 0, 0, 0};
+  Chunk c{base, before, 0, 0, 0, 0, 0, 0};
   if (i < a.B) {
-    const int q0 = min(max(a.q_starts[i], 0), a.T);
-    const int q1 = min(max(a.q_starts[i + 1], 0), a.T);
-    const int len = a.kv_lens[i];
-    const int rows = (q1 - q0) * a.G;
-    if (rows > 0) {
-      const int unit = 32 << a.unit_log2;
-      const bool broken =
-          len < 0 || len > ((long long)a.cols << a.page_log2);
-      c.one = OWN + (broken ? 0 : (len + unit - 1) / unit);
-      c.own = (rows + BM - 1) / BM * c.one;
+    c.q0 = min(max(a.q_starts[i], 0), a.T);
+    c.n = min(max(a.q_starts[i + 1], 0), a.T) - c.q0;
+    c.len = a.kv_lens[i];
+    if (c.len < 0 || c.len > ((long long)a.cols << a.page_log2)) c.len = -1;
+    if (c.n > 0) {
+      // at most 2^30 keys: the sum stays below 2^31
+      const int log2 = 5 + a.unit_log2;
+      c.one = OWN + ((max(c.len, 0) + (1 << log2) - 1) >> log2);
+      c.own = (c.n * a.G + BM - 1) / BM * c.one;
     }
   }
   c.upto = c.own;
@@ -397,17 +363,48 @@ __device__ inline Parts parts_of(const Line& l, long long first, int units) {
   return p;
 }
 
-__device__ inline Span span_of(const Args& a, int seq, int row0) {
+// the rows from row0 of sequence `seq`, one of the chunk's
+__device__ inline Span span_of(const Args& a, const Chunk& c, int seq,
+                               int row0) {
+  const int l = seq - c.base;
   Span s;
   s.seq = seq;
-  s.q0 = min(max(a.q_starts[seq], 0), a.T);
-  s.n = min(max(a.q_starts[seq + 1], 0), a.T) - s.q0;
+  s.q0 = __builtin_amdgcn_readlane(c.q0, l);
+  s.n = __builtin_amdgcn_readlane(c.n, l);
   s.rows = s.n * a.G;
   s.row0 = row0;
-  s.len = a.kv_lens[seq];
-  s.broken = s.len < 0 || s.len > ((long long)a.cols << a.page_log2);
-  if (s.broken) s.len = 0;
+  s.len = __builtin_amdgcn_readlane(c.len, l);
+  s.broken = s.len < 0;
+  s.len = max(s.len, 0);
   return s;
+}
+
+// Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
+// leaves each at least its own number, needs no sum over the sequences
+// before it, and the last such start at or below `tile` is its sequence.
+__device__ inline Span find(const Args& a, Chunk& c, int tile, int BM) {
+  Span s;
+  while (true) {
+    const int lane = threadIdx.x & 63;
+    const int first = c.q0 * a.G / BM + c.base + lane;
+    const unsigned long long at =
+        __ballot(c.base + lane < a.B && first <= tile);
+    if (at == 0) return s;
+    const int last = 63 - __clzll(at);
+    // the next chunk's first sequence may start at or below the tile as well
+    if (last == 63 && c.base + 64 < a.B) {
+      const int q0 = min(max(a.q_starts[c.base + 64], 0), a.T);
+      if (q0 * a.G / BM + c.base + 64 <= tile) {
+        c = chunk_of(a, c.base + 64,
+                     c.before + __builtin_amdgcn_readlane(c.upto, 63), BM);
+        continue;
+      }
+    }
+    const Span r = span_of(
+        a, c, c.base + last,
+        (tile - __builtin_amdgcn_readlane(first, last)) * BM);
+    return r.row0 < r.rows ? r : s;
+  }
 }
 
 // ---- the splits' parts ------------------------------------------------------
@@ -851,7 +848,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
     const long long start = (long long)h * line.head;
     const Item it = item_at(a, c, (int)(at - start), BM);
     if (it.seq < 0) return;
-    const Span s = span_of(a, it.seq, it.tile * BM);
+    const Span s = span_of(a, c, it.seq, it.tile * BM);
     const int from = (int)(at - start) - it.first;
     const int to = (int)min((long long)it.units, from + (end - at));
     // an item's last units may hold no key that its rows see
@@ -920,7 +917,8 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
-  const Span s = find(a, tile, BM);
+  Chunk c = chunk_of(a, 0, 0, BM);
+  const Span s = find(a, c, tile, BM);
   if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -1231,7 +1229,9 @@ __global__ void __launch_bounds__(256)
 join_kernel(Args a, int BM, int BN, int least) {
   constexpr int ROWS = 256 / (D / 4) / GS;
   const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
-  const Span s = find(a, tile, BM);
+  Chunk c;
+  const Line line = line_of(a, c, BM);
+  const Span s = find(a, c, tile, BM);
   if (s.seq < 0) return;
   Parts p;
   if (BN) {
@@ -1241,11 +1241,6 @@ join_kernel(Args a, int BM, int BN, int least) {
     p.part1 = p.part0 + 1;
     p.stride = 1;
   } else {
-    Chunk c;
-    const Line line = line_of(a, c, BM);
-    while (c.base + 64 <= s.seq)
-      c = chunk_of(a, c.base + 64,
-                   c.before + __builtin_amdgcn_readlane(c.upto, 63), BM);
     const int l = s.seq - c.base;
     const int units = __builtin_amdgcn_readlane(c.one, l);
     p = parts_of(line, (long long)h * line.head + c.before +
@@ -1338,7 +1333,7 @@ int tf_paged_attention(
       (workers && !join && (cols << page_log2) > (2 * NEAR - OWN) * 32) ||
       ((join || splits > 1) && !parts) ||
       ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
-      (long long)T * (Hq / Hk) >= (1LL << 31))
+      (long long)T * (Hq / Hk) + 128LL * B >= (1LL << 31))
     return (int)hipErrorInvalidValue;
   Args a{q, k, v, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
          (const int*)q_starts, (const int*)kv_lens, (const int*)table, out,

@@ -352,7 +352,7 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
         raise ValueError(f"{cols} pages of {cache.page_size} tokens: a "
                          "sequence has at most 2**30")
     G = Hq // Hk
-    if (T * G // 16 + B) * Hk >= 2 ** 31 or T * G >= 2 ** 31:
+    if (T * G // 16 + B) * Hk >= 2 ** 31 or T * G + 128 * B >= 2 ** 31:
         raise ValueError(f"{T} tokens of {Hq} heads: too many for a launch")
     scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
