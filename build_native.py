@@ -13,6 +13,8 @@ Artifacts:
   tf_accel_dump         accelerator ABI test driver (dlopen)
   libtfremote.so + tf_vgpu_worker  GPU-over-IP remoting (g++, dlopens HIP)
   libtftier.so          VRAM-tiering HIP kernels (hipcc --offload-arch=gfx950)
+  libtfops.so           decode, paged-cache and attention kernels (gfx950)
+  tf_paged.so           the paged operators' entry from Python
 
 The .so files are git-ignored but DO travel to the GPU box with gpurun.
 """
@@ -196,6 +198,32 @@ def build_fused_ops():
     return target
 
 
+def build_paged_binding():
+    """The paged operators' entry from Python, on libtfops.so."""
+
+    import sysconfig
+
+    import torch
+    src = os.path.join(NATIVE, "ops", "paged_binding.cpp")
+    ops = os.path.join(OUT, "libtfops.so")
+    if not os.path.exists(ops):
+        build_fused_ops()
+    target = os.path.join(OUT, "tf_paged.so")
+    if not _newer(target, [src, ops]):
+        return target
+    root = os.path.dirname(torch.__file__)
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          "-isystem", sysconfig.get_paths()["include"],
+          "-isystem", os.path.join(root, "include"),
+          "-isystem", os.path.join(ROCM, "include"), src, "-o", target,
+          "-L", OUT, "-ltfops", "-Wl,-rpath,$ORIGIN",
+          "-L", os.path.join(root, "lib"), "-lc10", "-lc10_hip",
+          "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+    return target
+
+
 ALL = {
     "limiter": build_limiter,
     "mockhip": build_mockhip,
@@ -206,6 +234,7 @@ ALL = {
     "remoting": build_remoting,
     "tiering": build_tiering,
     "fused_ops": build_fused_ops,
+    "paged_binding": build_paged_binding,
     "bw_sweep": build_bw_sweep,
 }
 

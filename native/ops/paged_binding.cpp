@@ -1,0 +1,543 @@
+// The paged operators' entry from Python: checks, outputs, workspaces and the
+// launch in one call of about 5 us, of which the launch itself is 3. (Through
+// ctypes, with the checks in Python, rope_kv_write took 15 us a call, five
+// times what its kernel takes for a decode step.)
+//
+// Everything that can be known without waiting for the GPU is checked here,
+// before anything is launched: a ValueError, or a RuntimeError where a
+// gradient is asked for. No C++ exception leaves a function.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/hip/HIPGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <new>
+#include <sstream>
+#include <stdexcept>
+#include <string>
+
+extern "C" {
+int tf_paged_write(const void* q, const void* k, const void* v,
+                   long long q_row, long long k_row, long long k_head,
+                   long long v_row, long long v_head, const void* cos_t,
+                   const void* sin_t, const void* pos, int positions,
+                   const void* slots, void* q_out, void* k_pool, void* v_pool,
+                   void* k_scale, void* v_scale, long long pages,
+                   int page_log2, int n, int heads, int kv_heads, int D,
+                   int fp16, void* stream);
+int tf_paged_read(const void* k_pool, const void* v_pool, const void* k_scale,
+                  const void* v_scale, long long pages, int page_log2,
+                  const void* slots, void* k, void* v, int n, int kv_heads,
+                  int D, int fp16, void* stream);
+int tf_paged_attention(
+    const void* q, const void* k, const void* v, const void* k_scale,
+    const void* v_scale, const void* q_starts, const void* kv_lens,
+    const void* table, void* out, void* parts, long long q_row,
+    long long q_head, long long table_row, int cols, int T, int B, int Hq,
+    int Hk, int pages, int page_log2, int D, float scale, int causal,
+    int fp16, int workers, int join, int splits, void* stream);
+}
+
+namespace {
+
+using at::Tensor;
+
+struct NoBackward : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+template <typename... A>
+[[noreturn]] void refuse(const A&... parts) {
+  std::ostringstream s;
+  (s << ... << parts);
+  throw std::invalid_argument(s.str());
+}
+
+struct Shape {
+  at::IntArrayRef of;
+};
+Shape shape(const Tensor& t) { return {t.sizes()}; }
+std::ostream& operator<<(std::ostream& s, const Shape& x) {
+  s << "(";
+  for (size_t i = 0; i < x.of.size(); ++i) s << (i ? ", " : "") << x.of[i];
+  return s << ")";
+}
+
+// ---- the pools of a cache -----------------------------------------------------
+
+struct Pools {
+  Tensor k, v, k_scale, v_scale;
+  int64_t pages;
+  int kv_heads, page_log2, D;
+  bool quantized;
+  at::ScalarType dtype;
+  at::Device device{at::kCPU};
+};
+
+struct PoolsObject {
+  PyObject_HEAD
+  Pools p;
+};
+
+PyTypeObject* pools_type = nullptr;
+
+bool wide(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+Tensor tensor_of(PyObject* o, const char* name) {
+  if (!THPVariable_Check(o)) refuse(name, " is a tensor");
+  Tensor t = THPVariable_Unpack(o);
+  if (t.layout() != at::kStrided) refuse(name, " is a dense tensor");
+  return t;
+}
+
+bool aligned(const Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+void check_pools(Pools& p) {
+  const Tensor &k = p.k, &v = p.v;
+  if (k.dim() != 4 || k.sizes() != v.sizes())
+    refuse("k and v pools are [pages, kv_heads, page_size, head_dim], of one "
+           "shape: got ", shape(k), " and ", shape(v));
+  const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2),
+                D = k.size(3);
+  if (D != 32 && D != 64 && D != 128)
+    refuse("head_dim is one of (32, 64, 128): ", D);
+  if (page < 16 || page > 1024 || (page & (page - 1)))
+    refuse("page_size is a power of two from 16 to 1024: ", page);
+  if (pages < 1 || heads < 1 || heads > 4096)
+    refuse("no pool of ", pages, " pages, ", heads, " heads");
+  if (pages >= (1LL << 31) / page)
+    refuse(pages, " pages of ", page, " tokens: a pool holds less than 2**31 "
+           "tokens");
+  p.dtype = k.scalar_type();
+  p.quantized = p.dtype == at::kFloat8_e4m3fn;
+  if ((!p.quantized && !wide(p.dtype)) || v.scalar_type() != p.dtype)
+    refuse("pools are both bfloat16, float16 or float8_e4m3fn: got ", p.dtype,
+           ", ", v.scalar_type());
+  for (const Tensor* s : {&p.k_scale, &p.v_scale}) {
+    if (!p.quantized) {
+      if (s->defined()) refuse("a ", p.dtype, " pool has no scales");
+    } else if (!s->defined() || s->scalar_type() != at::kByte ||
+               s->sizes() != k.sizes().slice(0, 3)) {
+      refuse("a float8_e4m3fn pool has a uint8 scale of shape ",
+             Shape{k.sizes().slice(0, 3)});
+    }
+  }
+  for (const Tensor* x : {&p.k, &p.v, &p.k_scale, &p.v_scale})
+    if (x->defined() && (!x->is_contiguous() || !aligned(*x) ||
+                         x->device() != k.device()))
+      refuse("pools and scales lie on one device, without gaps, at multiples "
+             "of 16 bytes");
+  p.pages = pages;
+  p.kv_heads = (int)heads;
+  p.page_log2 = __builtin_ctzll(page);
+  p.D = (int)D;
+  p.device = k.device();
+}
+
+const Pools& pools_of(PyObject* o) {
+  if (!PyObject_TypeCheck(o, pools_type)) refuse("a PagedKVCache is wanted");
+  return reinterpret_cast<PoolsObject*>(o)->p;
+}
+
+// ---- what the operators ask of their arguments --------------------------------
+
+void on_gpu(const Pools& p, std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all)
+    if (t->device() != p.device)
+      refuse("tensors on ", t->device(), " and a cache on ", p.device);
+  if (!p.device.is_cuda())
+    refuse("the paged operators run on a GPU: got ", p.device);
+}
+
+void no_grad(std::initializer_list<const Tensor*> all) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : all)
+    if (t->requires_grad())
+      throw NoBackward("the paged operators have no backward pass: call them "
+                       "under torch.no_grad()");
+}
+
+void check_rows(const Pools& p, std::initializer_list<const Tensor*> all) {
+  const at::ScalarType t = (*all.begin())->scalar_type();
+  if (!wide(t)) refuse("rows are bfloat16 or float16: got ", t);
+  if (!p.quantized && t != p.dtype)
+    refuse(t, " rows for a ", p.dtype, " cache");
+  for (const Tensor* x : all)
+    if (x->scalar_type() != t)
+      refuse("rows of one type: got ", t, ", ", x->scalar_type());
+}
+
+void check_index(const char* name, const Tensor& x, int64_t n) {
+  if (x.scalar_type() != at::kLong || x.dim() != 1 || x.size(0) != n ||
+      !x.is_contiguous())
+    refuse(name, " is int64 [", n, "] without gaps: got ", x.scalar_type(),
+           " ", shape(x));
+}
+
+// x, or a copy of it where 16-byte loads do not fit its layout
+Tensor rows_of(const Tensor& x) {
+  bool fits = x.stride(-1) == 1 && aligned(x);
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) fits = fits && x.stride(i) % 8 == 0;
+  return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+void* stream_of(const Pools& p) {
+  return c10::hip::getCurrentHIPStream(p.device.index()).stream();
+}
+
+void launched(const char* name, int rc) {
+  if (rc)
+    throw std::runtime_error(std::string(name) + " failed: " +
+                             std::to_string(rc));
+}
+
+void write(const Pools& p, const Tensor& q, const Tensor& k, const Tensor& v,
+           int64_t k_head, int64_t v_head, const Tensor& cos,
+           const Tensor& sin, const Tensor& pos, const Tensor& slots,
+           const Tensor& q_out, int n, int heads) {
+  launched("tf_paged_write",
+           tf_paged_write(
+               ptr(q), ptr(k), ptr(v), q.defined() ? q.stride(0) : 0,
+               k.stride(0), k_head, v.stride(0), v_head, ptr(cos), ptr(sin),
+               ptr(pos), cos.defined() ? (int)cos.size(0) : 0, ptr(slots),
+               ptr(q_out), ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale),
+               p.pages, p.page_log2, n, heads, p.kv_heads, p.D,
+               k.scalar_type() == at::kHalf, stream_of(p)));
+}
+
+void kv_write(const Pools& p, Tensor k, Tensor v, const Tensor& slots) {
+  const int64_t n = k.dim() ? k.size(0) : 0;
+  const int64_t want[] = {n, p.kv_heads, p.D};
+  if (k.sizes() != at::IntArrayRef(want) || v.sizes() != at::IntArrayRef(want))
+    refuse("k and v are ", Shape{want}, ": got ", shape(k), " and ", shape(v));
+  check_rows(p, {&k, &v});
+  check_index("slots", slots, n);
+  no_grad({&k, &v});
+  on_gpu(p, {&k, &v, &slots});
+  if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
+  if (n == 0) return;
+  const c10::DeviceGuard guard(p.device);
+  k = rows_of(k);
+  v = rows_of(v);
+  write(p, Tensor(), k, v, k.stride(1), v.stride(1), Tensor(), Tensor(),
+        Tensor(), slots, Tensor(), (int)n, 0);
+}
+
+Tensor rope_kv_write(const Pools& p, Tensor q_in, Tensor k_in, Tensor v_in,
+                     const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                     const Tensor& slots, int64_t heads) {
+  const int64_t n = q_in.dim() ? q_in.size(0) : 0, D = p.D;
+  if (heads < 1 || heads > 65535 || q_in.dim() != 2 ||
+      q_in.size(1) != heads * D)
+    refuse("q_in is [n, ", heads, " * ", D, "]: got ", shape(q_in));
+  const int64_t want[] = {n, p.kv_heads * D};
+  if (k_in.sizes() != at::IntArrayRef(want) ||
+      v_in.sizes() != at::IntArrayRef(want))
+    refuse("k_in and v_in are ", Shape{want}, ": got ", shape(k_in), " and ",
+           shape(v_in));
+  check_rows(p, {&q_in, &k_in, &v_in});
+  for (const Tensor* x : {&cos, &sin})
+    if (x->scalar_type() != at::kFloat || x->dim() != 2 || x->size(0) < 1 ||
+        x->size(0) >= (1LL << 31) || x->sizes() != cos.sizes() ||
+        x->size(1) != D / 2 || !x->is_contiguous() || !aligned(*x))
+      refuse("cos and sin are float32 [positions, ", D / 2, "] without gaps");
+  check_index("pos", pos, n);
+  check_index("slots", slots, n);
+  if (heads + 2 * p.kv_heads > 65535 || n >= (1LL << 31))
+    refuse("too many heads (", heads, ") or rows (", n, ")");
+  no_grad({&q_in, &k_in, &v_in});
+  on_gpu(p, {&q_in, &k_in, &v_in, &cos, &sin, &pos, &slots});
+  const c10::DeviceGuard guard(p.device);
+  Tensor q = at::empty({n, heads, D}, q_in.options().requires_grad(false));
+  if (n == 0) return q;
+  q_in = rows_of(q_in);
+  k_in = rows_of(k_in);
+  v_in = rows_of(v_in);
+  write(p, q_in, k_in, v_in, D, D, cos, sin, pos, slots, q, (int)n,
+        (int)heads);
+  return q;
+}
+
+std::pair<Tensor, Tensor> kv_read(const Pools& p, const Tensor& slots,
+                                  at::ScalarType dtype) {
+  if (!wide(dtype) || !(p.quantized || dtype == p.dtype))
+    refuse("a ", p.dtype, " cache is not read as ", dtype);
+  if (slots.dim() != 1) refuse("slots is int64 [n]: got ", shape(slots));
+  const int64_t n = slots.size(0);
+  check_index("slots", slots, n);
+  on_gpu(p, {&slots});
+  if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
+  const c10::DeviceGuard guard(p.device);
+  const auto options = p.k.options().dtype(dtype);
+  Tensor k = at::empty({n, p.kv_heads, p.D}, options);
+  Tensor v = at::empty({n, p.kv_heads, p.D}, options);
+  if (n)
+    launched("tf_paged_read",
+             tf_paged_read(ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale),
+                           p.pages, p.page_log2, ptr(slots), ptr(k), ptr(v),
+                           (int)n, p.kv_heads, p.D, dtype == at::kHalf,
+                           stream_of(p)));
+  return {k, v};
+}
+
+struct Plan {
+  int64_t workers, join, splits;
+};
+
+// Which kernel attends, and how it shares the keys. What a batch holds lies
+// on the device; this goes by its mean, and is right for any batch. Up to 16
+// rows (new tokens * G) a sequence are work for the kernel for few rows, whose
+// `workers` share it out among themselves; 0 workers: the kernel for many
+// rows, with the keys of each tile of 128 rows in `splits` parts.
+Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t keys) {
+  const int64_t rows = T * G;
+  // of keys that are worth a workgroup
+  const int64_t pieces = std::max<int64_t>(1, (keys + 255) / 256);
+  if (rows <= 16 * B) {
+    // two workgroups fit a unit; neighbouring ones share an XCD of eight
+    const int64_t items = Hk * std::max(B, rows / 16);
+    const int64_t workers = std::min<int64_t>(512, items * pieces);
+    return {(workers + 7) / 8 * 8, keys > 384, 1};  // 384: never split
+  }
+  const int64_t busy = Hk * std::max(B, rows / 128);
+  return {0, 0, std::min(pieces, std::max<int64_t>(1, 512 / busy))};
+}
+
+Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
+                 const Tensor& lens, const Tensor& table, double scale,
+                 bool causal, Tensor out) {
+  if (q.dim() != 3) refuse("q is [tokens, heads, head_dim]: ", shape(q));
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2),
+                Hk = p.kv_heads;
+  if (D != p.D || Hq < 1 || Hq % Hk)
+    refuse("q ", shape(q), " for a cache of ", Hk, " heads of ", p.D);
+  check_rows(p, {&q});
+  if (lens.dim() != 1 || table.dim() != 2 || starts.dim() != 1)
+    refuse("q_starts is [B + 1], kv_lens is [B], block_table [B, columns]");
+  const int64_t B = table.size(0), cols = table.size(1);
+  if (lens.size(0) != B || starts.size(0) != B + 1)
+    refuse("for ", B, " sequences of the table: kv_lens ", shape(lens),
+           ", q_starts ", shape(starts));
+  for (const Tensor* x : {&starts, &lens, &table})
+    if (x->scalar_type() != at::kInt)
+      refuse("q_starts, kv_lens and block_table are int32");
+  if (!starts.is_contiguous() || !lens.is_contiguous() ||
+      (cols > 1 && table.stride(1) != 1))
+    refuse("q_starts, kv_lens and the table's rows have no gaps");
+  if (cols > (1LL << 30) >> p.page_log2)
+    refuse(cols, " pages of ", 1 << p.page_log2, " tokens: a sequence has at "
+           "most 2**30");
+  const int64_t G = Hq / Hk, most = 1LL << 31;
+  if (T >= most || B >= most || T * G + 128 * B >= most ||
+      (T * G / 16 + B) * Hk >= most)
+    refuse(T, " tokens of ", Hq, " heads: too many for a launch");
+  if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)D);
+  no_grad({&q});
+  on_gpu(p, {&q, &starts, &lens, &table});
+  if (!out.defined())
+    out = at::empty({T, Hq, D}, q.options().requires_grad(false));
+  else if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() ||
+           !out.is_contiguous() || out.device() != q.device() ||
+           !aligned(out))
+    refuse("out has q's shape, type and device, without gaps");
+  else
+    no_grad({&out});
+  if (T == 0 || B == 0) return out;
+  const c10::DeviceGuard guard(p.device);
+  q = rows_of(q);
+  const Plan plan = plan_of(T, B, G, Hk, cols << p.page_log2);
+  Tensor parts;
+  if (plan.join || plan.splits > 1) {
+    // its own for every call: two captured graphs never share it
+    const int64_t rows = plan.workers
+                             ? 2 * plan.workers * 16
+                             : (T * G / 128 + B) * Hk * plan.splits * 128;
+    parts = at::empty({rows * (D + 2)},
+                      q.options().dtype(at::kFloat).requires_grad(false));
+  }
+  launched("tf_paged_attention",
+           tf_paged_attention(
+               ptr(q), ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale),
+               ptr(starts), ptr(lens), ptr(table), ptr(out), ptr(parts),
+               q.stride(0), q.stride(1), table.stride(0), (int)cols, (int)T,
+               (int)B, (int)Hq, (int)Hk, (int)p.pages, p.page_log2, (int)D,
+               (float)scale, causal, q.scalar_type() == at::kHalf,
+               (int)plan.workers, (int)plan.join, (int)plan.splits,
+               stream_of(p)));
+  return out;
+}
+
+// ---- from and to Python --------------------------------------------------------
+
+template <typename F>
+PyObject* guarded(F f) {
+  try {
+    return f();
+  } catch (const std::invalid_argument& e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type =
+        torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    PyErr_SetString(type ? type : PyExc_RuntimeError,
+                    e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+  } catch (const c10::Error& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+  }
+  return nullptr;
+}
+
+void count(Py_ssize_t got, Py_ssize_t want) {
+  if (got != want) refuse(want, " arguments are wanted: got ", got);
+}
+
+int64_t int_of(PyObject* o, const char* name) {
+  const long long x = PyLong_AsLongLong(o);
+  if (x == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(name, " is a whole number");
+  }
+  return x;
+}
+
+PyObject* py_pools(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 4);
+    Pools p;
+    p.k = tensor_of(a[0], "k");
+    p.v = tensor_of(a[1], "v");
+    if (a[2] != Py_None) p.k_scale = tensor_of(a[2], "k_scale");
+    if (a[3] != Py_None) p.v_scale = tensor_of(a[3], "v_scale");
+    check_pools(p);
+    auto* o = reinterpret_cast<PoolsObject*>(
+        pools_type->tp_alloc(pools_type, 0));
+    if (!o) return nullptr;
+    new (&o->p) Pools(std::move(p));
+    return reinterpret_cast<PyObject*>(o);
+  });
+}
+
+void pools_dealloc(PyObject* o) {
+  PyTypeObject* type = Py_TYPE(o);
+  reinterpret_cast<PoolsObject*>(o)->p.~Pools();
+  type->tp_free(o);
+  Py_DECREF(type);
+}
+
+PyObject* py_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 4);
+    kv_write(pools_of(a[0]), tensor_of(a[1], "k"), tensor_of(a[2], "v"),
+             tensor_of(a[3], "slots"));
+    Py_RETURN_NONE;
+  });
+}
+
+PyObject* py_rope_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 9);
+    return THPVariable_Wrap(rope_kv_write(
+        pools_of(a[0]), tensor_of(a[1], "q_in"), tensor_of(a[2], "k_in"),
+        tensor_of(a[3], "v_in"), tensor_of(a[4], "cos"),
+        tensor_of(a[5], "sin"), tensor_of(a[6], "pos"),
+        tensor_of(a[7], "slots"), int_of(a[8], "heads")));
+  });
+}
+
+PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 3);
+    const Pools& p = pools_of(a[0]);
+    at::ScalarType t = p.quantized ? at::kBFloat16 : p.dtype;
+    if (a[2] != Py_None) {
+      if (!THPDtype_Check(a[2])) refuse("dtype is a torch.dtype");
+      t = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
+    }
+    auto kv = kv_read(p, tensor_of(a[1], "slots"), t);
+    PyObject* k = THPVariable_Wrap(kv.first);
+    PyObject* v = THPVariable_Wrap(kv.second);
+    PyObject* r = k && v ? PyTuple_Pack(2, k, v) : nullptr;
+    Py_XDECREF(k);
+    Py_XDECREF(v);
+    return r;
+  });
+}
+
+PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 8);
+    double scale = std::nan("");
+    if (a[5] != Py_None) {
+      scale = PyFloat_AsDouble(a[5]);
+      if (PyErr_Occurred()) return nullptr;
+      if (!std::isfinite((float)scale))
+        refuse("scale is a finite number: got ", scale);
+    }
+    const int causal = PyObject_IsTrue(a[6]);
+    if (causal < 0) return nullptr;
+    Tensor out;
+    if (a[7] != Py_None) out = tensor_of(a[7], "out");
+    return THPVariable_Wrap(attention(
+        pools_of(a[0]), tensor_of(a[1], "q"), tensor_of(a[2], "q_starts"),
+        tensor_of(a[3], "kv_lens"), tensor_of(a[4], "block_table"), scale,
+        causal, out));
+  });
+}
+
+PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 5);
+    const Plan p = plan_of(int_of(a[0], "T"), int_of(a[1], "B"),
+                           int_of(a[2], "G"), int_of(a[3], "Hk"),
+                           int_of(a[4], "keys"));
+    return Py_BuildValue("LLL", (long long)p.workers, (long long)p.join,
+                         (long long)p.splits);
+  });
+}
+
+#define TF_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
+PyMethodDef methods[] = {
+    {"pools", TF_FAST(py_pools), METH_FASTCALL, nullptr},
+    {"kv_write", TF_FAST(py_kv_write), METH_FASTCALL, nullptr},
+    {"rope_kv_write", TF_FAST(py_rope_kv_write), METH_FASTCALL, nullptr},
+    {"kv_read", TF_FAST(py_kv_read), METH_FASTCALL, nullptr},
+    {"attention", TF_FAST(py_attention), METH_FASTCALL, nullptr},
+    {"plan", TF_FAST(py_plan), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "tf_paged", nullptr, -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
+
+PyType_Slot pools_slots[] = {{Py_tp_dealloc, (void*)pools_dealloc},
+                             {0, nullptr}};
+PyType_Spec pools_spec = {"tf_paged.Pools", sizeof(PoolsObject), 0,
+                          Py_TPFLAGS_DEFAULT | Py_TPFLAGS_DISALLOW_INSTANTIATION,
+                          pools_slots};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_tf_paged() {
+  PyObject* m = PyModule_Create(&module);
+  if (!m) return nullptr;
+  pools_type = reinterpret_cast<PyTypeObject*>(PyType_FromSpec(&pools_spec));
+  if (!pools_type) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -4,6 +4,8 @@ import torch
 
 from tensor_fusion_amd.ops import paged
 
+pytestmark = pytest.mark.usefixtures("native_built")
+
 
 def cache(dtype=torch.bfloat16, quantized=False, D=64, page=16, Hk=2, pages=5):
     return paged.make_cache(pages, page, Hk, D, dtype, quantized,
@@ -54,7 +56,8 @@ def test_cache_refusals():
 def test_quantized_cache_starts_at_zero():
     c = cache(quantized=True)
     assert c.quantized and c.k.float().abs().sum() == 0
-    assert (c.k_scale == 127).all() and c.page_log2 == 4
+    assert (c.k_scale == 127).all()
+    assert (c.pages, c.kv_heads, c.page_size, c.head_dim) == (5, 2, 16, 64)
 
 
 def test_write_refusals():
@@ -149,7 +152,7 @@ def test_attention_refusals():
 def test_plan_covers_every_row(T, B, G):
     """Whatever the lengths, each sequence's tiles fit the grid."""
 
-    workers, join, splits = paged._plan(T, B, G, 8, 4096)
+    workers, join, splits = paged._ext().plan(T, B, G, 8, 4096)
     assert 1 <= splits <= 16
     assert workers == 0 or (join and 8 <= workers <= 512
                             and workers % 8 == 0)
