@@ -208,15 +208,15 @@ __device__ inline u4 finite_only(Oct<K> o) {
   return o.raw;
 }
 
-// Calls add(d, v) for each value v = row[d] of a key's V row in LDS that is
-// NaN or infinite, d and v the wave's. place(d): where value d lies.
-template <typename K, int D, typename P, typename F>
-__device__ inline void each_strange(P place, F add) {
+// Calls add(d, v) for each value v = at(d) of a key's V row that is NaN or
+// infinite, d and v the wave's.
+template <int D, typename P, typename F>
+__device__ inline void each_strange(P at, F add) {
   const int lane = threadIdx.x & 63;
 #pragma unroll 1
   for (int d0 = 0; d0 < D; d0 += 64) {
     const int d = d0 + lane;
-    float v = d < D ? (float)*place(d) : 0.0f;
+    float v = d < D ? at(d) : 0.0f;
     unsigned long long found = __ballot(!(fabsf(v) < plus_inf()));
     while (found) {
       const int i = __ffsll(found) - 1;
@@ -730,10 +730,11 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
       // what is not finite goes to the rows that see it, then gives way
 #pragma unroll 1
       for (int key = 0; key < BN; ++key)
-        each_strange<K, D>(
+        each_strange<D>(
             [&](int d) {
-              return (const T*)(mine_v + key * (D * 2) +
-                                few_piece<D>(key, d >> 3) * 16 + (d & 7) * 2);
+              return (float)*(const T*)(mine_v + key * (D * 2) +
+                                        few_piece<D>(key, d >> 3) * 16 +
+                                        (d & 7) * 2);
             },
             [&](int d, float v) {
 #pragma unroll
@@ -892,8 +893,9 @@ __device__ inline void to_lds(const void* base, uint32_t off, uint32_t to) {
       : "v"(off), "s"(base), "s"(to)
       : "memory");
 }
+template <int LATER>  // loads that were issued later
 __device__ inline void landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
 }
 __device__ inline uint32_t lds_address(const void* p) {
   return (uint32_t)(size_t)(const __attribute__((address_space(3))) char*)p;
@@ -911,9 +913,9 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   constexpr int NL = ROWS >= 16 ? 1 : 16 / ROWS;  // loads for its 16 rows
   constexpr int TILE = BN * D * 2;      // bytes of a tile in LDS
 
-  // K, V of one tile, then of the next
+  // K of two tiles, V of two
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  __shared__ int odd_tile[2];  // the last tile here whose V is strange, + 1
+  __shared__ int odd_v;  // whether a V value was not finite where it matters
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
@@ -929,7 +931,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
                               4);
   if ((int)blockIdx.y >= mine.active) return;
-  if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+  if (threadIdx.x == 0) odd_v = 0;
   __syncthreads();
 
   // this wave's rows
@@ -965,6 +967,12 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
     return kt < mine.last && key < seen_max
                ? uniform_load(pages + (key >> a.page_log2)) : 0;
   };
+  auto row_of = [&](int id, int kt) {
+    const bool bad = (unsigned)id >= (unsigned)a.pages;
+    const int key = kt * BN + wave * 16;
+    return (((long long)(bad ? 0 : id) * a.Hk + h) << a.page_log2) +
+           (key & in_page);
+  };
   uint32_t k_off[NL], v_off[NL];  // 16 bits: what a lane brings of 16 rows
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
@@ -975,39 +983,80 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   u4 kr[NL], vr[NL];  // 8 bits: codes on their way
   uint32_t ksr[NL], vsr[NL];
   const bool loads = lrow < 16;
-  const uint32_t lds0 = lds_address(lds);
-  int id = 0, bad = 0;
+  const uint32_t lds0 = lds_address(lds) + wave * (TILE / 4);
+  // tile kt's K at (kt & 1) * TILE, its V behind both K's; this wave's rows
+  auto k_tile = [&](int kt) { return lds + (kt & 1) * TILE; };
+  auto v_tile = [&](int kt) { return lds + (2 + (kt & 1)) * TILE; };
 
-  auto fetch = [&](int kt) {
-    bad = (unsigned)id >= (unsigned)a.pages;
-    const int key = kt * BN + wave * 16;
-    const long long row =
-        (((long long)(bad ? 0 : id) * a.Hk + h) << a.page_log2) +
-        (key & in_page);
-    const char* ks = (const char*)a.k + row * (D * EB);
-    const char* vs = (const char*)a.v + row * (D * EB);
+  auto fetch_k = [&](int id, int kt) {
+    const long long row = row_of(id, kt);
+    const char* src = (const char*)a.k + row * (D * EB);
     if constexpr (Q8) {
       if (loads)
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int at = i * ROWS + lrow;
-          kr[i] = *reinterpret_cast<const u4*>(ks + at * D + lpos * 16);
-          vr[i] = *reinterpret_cast<const u4*>(vs + at * D + lpos * 16);
+          kr[i] = *reinterpret_cast<const u4*>(src + at * D + lpos * 16);
           ksr[i] = a.k_scale[row + at];
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        to_lds(src, k_off[i], lds0 + (kt & 1) * TILE + i * 1024);
+    }
+  };
+  auto fetch_v = [&](int id, int kt) {
+    const long long row = row_of(id, kt);
+    const char* src = (const char*)a.v + row * (D * EB);
+    if constexpr (Q8) {
+      if (loads)
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int at = i * ROWS + lrow;
+          vr[i] = *reinterpret_cast<const u4*>(src + at * D + lpos * 16);
           vsr[i] = a.v_scale[row + at];
         }
     } else {
-      const uint32_t to = lds0 + (kt & 1) * (2 * TILE) + wave * (TILE / 4);
 #pragma unroll
-      for (int i = 0; i < NL; ++i) to_lds(ks, k_off[i], to + i * 1024);
-#pragma unroll
-      for (int i = 0; i < NL; ++i) to_lds(vs, v_off[i], to + TILE + i * 1024);
+      for (int i = 0; i < NL; ++i)
+        to_lds(src, v_off[i], lds0 + (2 + (kt & 1)) * TILE + i * 1024);
     }
   };
-  // what fetch brought becomes the tile, but for the barrier
-  auto put = [&](int kt) {
-    char* kd = lds + (kt & 1) * (2 * TILE) + wave * (TILE / 4);
-    char* vd = kd + TILE;
+  // What was fetched becomes the tile, but for the barrier. `more`: NL loads
+  // to LDS that were issued later may still be on their way. A key without
+  // a page scores NaN: its K row is NaN, its V row 0. V rows past the end
+  // are 0, and where rows of the tile see different keys, values that are
+  // not finite are 0 too: they are seen to behind the loop.
+  auto put_k = [&](int id, int kt, bool more) {
+    const bool bad = (unsigned)id >= (unsigned)a.pages;
+    char* to = k_tile(kt) + wave * (TILE / 4);
+    if constexpr (Q8) {
+      if (!loads) return;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int row = i * ROWS + lrow, c = lpos * 2, at = wave * 16 + row;
+        if (bad) kr[i] = u4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu,
+                            0x7f7f7f7fu};
+        Oct<K> x, y;
+        const float sc = scale_of(ksr[i]);
+        widen(x, u2{kr[i][0], kr[i][1]}, sc);
+        widen(y, u2{kr[i][2], kr[i][3]}, sc);
+        char* r = to + row * (D * 2);
+        *reinterpret_cast<u4*>(r + k_piece<D>(at, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(r + k_piece<D>(at, c + 1) * 16) = y.raw;
+      }
+    } else {
+      if (more) landed<NL>(); else landed<0>();
+      if (!bad) return;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        *reinterpret_cast<u4*>(to + i * 1024 + lane * 16) =
+            u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+    }
+  };
+  auto put_v = [&](int id, int kt, bool more) {
+    const bool bad = (unsigned)id >= (unsigned)a.pages;
+    char* to = v_tile(kt) + wave * (TILE / 4);
     const int key0 = kt * BN + wave * 16;
     const bool past = key0 + 16 > seen_max;
     const bool cut = (kt + 1) * BN > seen_min;
@@ -1016,44 +1065,37 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
       if (!loads) return;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int row = i * ROWS + lrow, c = lpos * 2;
-        const bool there = !bad && (!past || key0 + row < seen_max);
-        // a key without a page scores NaN: its K row is NaN, its V row 0
-        if (bad) kr[i] = u4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu,
-                            0x7f7f7f7fu};
+        const int row = i * ROWS + lrow, c = lpos * 2, at = wave * 16 + row;
         Oct<K> x, y;
-        float sc = scale_of(ksr[i]);
-        widen(x, u2{kr[i][0], kr[i][1]}, sc);
-        widen(y, u2{kr[i][2], kr[i][3]}, sc);
-        char* to = kd + row * (D * 2);
-        const int at = wave * 16 + row;
-        *reinterpret_cast<u4*>(to + k_piece<D>(at, c) * 16) = x.raw;
-        *reinterpret_cast<u4*>(to + k_piece<D>(at, c + 1) * 16) = y.raw;
-        sc = scale_of(vsr[i]);
+        const float sc = scale_of(vsr[i]);
         widen(x, u2{vr[i][0], vr[i][1]}, sc);
         widen(y, u2{vr[i][2], vr[i][3]}, sc);
-        if (!there) x.raw = y.raw = u4{0, 0, 0, 0};
-        odd |= strange(x) || strange(y);
-        to = vd + row * (D * 2);
-        *reinterpret_cast<u4*>(to + v_piece_at<D>(at, c) * 16) = x.raw;
-        *reinterpret_cast<u4*>(to + v_piece_at<D>(at, c + 1) * 16) = y.raw;
+        if (bad || (past && key0 + row >= seen_max))
+          x.raw = y.raw = u4{0, 0, 0, 0};
+        if (cut && (strange(x) || strange(y))) {
+          odd = true;
+          x.raw = finite_only<K>(x);
+          y.raw = finite_only<K>(y);
+        }
+        char* r = to + row * (D * 2);
+        *reinterpret_cast<u4*>(r + v_piece_at<D>(at, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(r + v_piece_at<D>(at, c + 1) * 16) = y.raw;
       }
     } else {
-      landed();
+      if (more) landed<NL>(); else landed<0>();
       if (!bad && !cut) return;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < NL; ++i) {
-        Oct<K>* x = reinterpret_cast<Oct<K>*>(vd + i * 1024 + lane * 16);
-        if (bad || (past && key0 + i * ROWS + lrow >= seen_max))
+        Oct<K>* x = reinterpret_cast<Oct<K>*>(to + i * 1024 + lane * 16);
+        if (bad || (past && key0 + i * ROWS + lrow >= seen_max)) {
           x->raw = u4{0, 0, 0, 0};
-        else
-          odd |= strange(*x);
-        if (bad)
-          *reinterpret_cast<u4*>(kd + i * 1024 + lane * 16) =
-              u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+        } else if (strange(*x)) {
+          odd = true;
+          x->raw = finite_only<K>(*x);
+        }
       }
     }
-    if (odd) odd_tile[kt & 1] = kt + 1;
+    if (odd) odd_v = 1;
   };
 
   f16v o[NT];
@@ -1078,117 +1120,134 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
                 (lane & 1) * 8;
   }
 
+  // S^T of 32 keys, whose K rows start at kd
+  auto scores = [&](const char* kd, f16v& sc) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[j] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      Oct<K> x;
+      x.raw = *reinterpret_cast<const u4*>(kd + k_at[f]);
+      sc = mfma32(x.v, q[f].v, sc);
+    }
+  };
+  // The 32 keys from key0 join the sums, while the scores of the next 32 are
+  // worked out: what one needs of the vector pipe, the other does not. (Those
+  // of no keys at the end, from what lies there, are not used.)
+  auto step = [&](int key0, f16v& sc, const char* vd, const char* next_kd,
+                  f16v& next) {
+    if (key0 + 32 > wave_min) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int key = key0 + (j & 3) + 8 * (j >> 2) + 4 * hi;
+        if (key >= seen) sc[j] = minus_inf();
+      }
+    }
+    float top = sc[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
+    top = lane_xor32_max(top) * scale;
+    // The sums stay under an old maximum until a score is 2^8 above it:
+    // p is then at most 2^8, with the same relative rounding.
+    if (__ballot(top > m + 8.0f)) {
+      const float higher = fmaxf(m, top);
+      const float keep = exp2_of(m - base_of(higher));
+      m = higher;
+      sum *= keep;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] *= keep;
+    }
+    const float base = base_of(m);
+    scores(next_kd, next);
+    Oct<K> p[2];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      p[j >> 3].h[j & 7] =
+          (T)exp2_of(__builtin_fmaf(sc[j], scale, -base));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = add_pair(p[j >> 2], j & 3, sum);
+    // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const char* at = vd + v_at[t] + half * 16 * (D * 2);
+        const u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
+        Oct<K> x;
+        x.raw = u4{lo[0], lo[1], up[0], up[1]};
+        o[t] = mfma32(x.v, p[half].v, o[t]);
+      }
+  };
+  // K runs one tile ahead of its use, V half a tile less: each load to LDS
+  // has the time of a tile. Two barriers a tile: behind the first, K(kt + 1)
+  // is there and K(kt) is free; behind the second, V(kt + 1), and V(kt).
+  f16v s0, s1;
   int kt = mine.first;
-  id = page_of(kt);
+  int id1 = page_of(kt), id2 = page_of(kt + 1);  // of the next V, the next K
   if (kt < mine.last) {
-    fetch(kt);
-    id = page_of(kt + 1);
-    put(kt);
+    fetch_k(id1, kt);
+    put_k(id1, kt, false);
+    fetch_v(id1, kt);
+    put_v(id1, kt, false);
+    if (kt + 1 < mine.last) fetch_k(id2, kt + 1);
   }
   __syncthreads();
+  if (kt < mine.last && kt * BN < wave_max) scores(k_tile(kt), s0);
   for (; kt < mine.last; ++kt) {
-    const bool more = kt + 1 < mine.last;
-    if (more) {
-      fetch(kt + 1);
-      id = page_of(kt + 2);
-    }
+    const bool more = kt + 1 < mine.last, more2 = kt + 2 < mine.last;
     const int key0 = kt * BN;
-    const char* kd = lds + (kt & 1) * (2 * TILE);
-    char* vd = lds + (kt & 1) * (2 * TILE) + TILE;
-    const bool works = key0 < wave_max;
-    Oct<K> p[4];
-    if (works) {
-      f16v sc[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) sc[half][j] = 0.0f;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          Oct<K> x;
-          x.raw = *reinterpret_cast<const u4*>(kd + k_at[f] +
-                                               half * 32 * (D * 2));
-          sc[half] = mfma32(x.v, q[f].v, sc[half]);
-        }
-      }
-      const bool cut = key0 + BN > wave_min;
-      if (cut) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int key =
-                key0 + half * 32 + (j & 3) + 8 * (j >> 2) + 4 * hi;
-            if (key >= seen) sc[half][j] = minus_inf();
-          }
-      }
-      float top = sc[0][0];
-#pragma unroll
-      for (int j = 1; j < 32; ++j) top = fmaxf(top, sc[j >> 4][j & 15]);
-      top = lane_xor32_max(top) * scale;
-      // The sums stay under an old maximum until a score is 2^8 above it:
-      // p is then at most 2^8, with the same relative rounding.
-      if (__ballot(top > m + 8.0f)) {
-        const float next = fmaxf(m, top);
-        const float keep = exp2_of(m - base_of(next));
-        m = next;
-        sum *= keep;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[t][j] *= keep;
-      }
-      const float base = base_of(m);
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        p[j >> 3].h[j & 7] = (T)exp2_of(
-            __builtin_fmaf(sc[j >> 4][j & 15], scale, -base));
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        sum = add_pair(p[j >> 2], j & 3, sum);
+    id1 = id2;
+    id2 = page_of(kt + 2);
+    if constexpr (Q8) {
+      if (more) put_k(id1, kt + 1, false);
     }
-    if (key0 + BN > seen_min && odd_tile[kt & 1] == kt + 1) {
-      // what is not finite goes to the rows that see it, then gives way
-      if (works)
-#pragma unroll 1
-        for (int key = 0; key < BN; ++key)
-          each_strange<K, D>(
-              [&](int d) {
-                return (const T*)(vd + key * (D * 2) +
-                                  v_piece_at<D>(key, d >> 3) * 16 +
-                                  (d & 7) * 2);
-              },
-              [&](int d, float v) {
-#pragma unroll
-                for (int i = 0; i < NT * 16; ++i)
-                  if (d == (i >> 4) * 32 + (i & 3) + 8 * ((i & 15) >> 2) +
-                               4 * hi &&
-                      key0 + key < seen)
-                    o[i >> 4][i & 15] += v;
-              });
-      __syncthreads();
-#pragma unroll 1
-      for (int i = threadIdx.x; i < BN * D / 8; i += 256) {
-        Oct<K>* x = reinterpret_cast<Oct<K>*>(vd + i * 16);
-        x->raw = finite_only<K>(*x);
-      }
-      __syncthreads();
+    if (more) fetch_v(id1, kt + 1);
+    if (key0 < wave_max)
+      step(key0, s0, v_tile(kt), k_tile(kt) + 32 * (D * 2), s1);
+    if constexpr (!Q8) {
+      if (more) put_k(id1, kt + 1, true);
     }
-    if (works) {
-      // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
-#pragma unroll
-      for (int step = 0; step < 4; ++step)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const char* at = vd + v_at[t] + step * 16 * (D * 2);
-          u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
-          Oct<K> x;
-          x.raw = u4{lo[0], lo[1], up[0], up[1]};
-          o[t] = mfma32(x.v, p[step].v, o[t]);
-        }
-    }
-    if (more) put(kt + 1);
     __syncthreads();
+    if constexpr (Q8) {
+      if (more) put_v(id1, kt + 1, false);
+    }
+    if (more2) fetch_k(id2, kt + 2);
+    if (key0 + 32 < wave_max)
+      step(key0 + 32, s1, v_tile(kt) + 32 * (D * 2), k_tile(kt + 1), s0);
+    if constexpr (!Q8) {
+      if (more) put_v(id1, kt + 1, more2);
+    }
+    __syncthreads();
+  }
+
+  if (odd_v) {
+    // What is not finite, from memory again, to the rows that see it.
+#pragma unroll 1
+    for (int key = max(seen_min / BN, mine.first) * BN;
+         key < min(mine.last * BN, seen_max); ++key) {
+      const int id = uniform_load(pages + (key >> a.page_log2));
+      if ((unsigned)id >= (unsigned)a.pages) continue;
+      const long long row =
+          (((long long)id * a.Hk + h) << a.page_log2) + (key & in_page);
+      each_strange<D>(
+          [&](int d) {
+            if constexpr (Q8)
+              return (float)(T)(e4m3_values(((const uint8_t*)a.v)[row * D + d],
+                                            scale_of(a.v_scale[row]))[0]);
+            else
+              return (float)((const T*)a.v)[row * D + d];
+          },
+          [&](int d, float v) {
+#pragma unroll
+            for (int i = 0; i < NT * 16; ++i)
+              if (d == (i >> 4) * 32 + (i & 3) + 8 * ((i & 15) >> 2) +
+                           4 * hi &&
+                  key < seen)
+                o[i >> 4][i & 15] += v;
+          });
+    }
   }
 
   sum = lane_xor32_add(sum);
