@@ -1160,6 +1160,9 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
         for (int j = 0; j < 16; ++j) o[t][j] *= keep;
     }
     const float base = base_of(m);
+    // while this wave feeds the matrix pipe, the unit's other wave waits
+    // with its own products, and takes the vector pipe
+    __builtin_amdgcn_s_setprio(1);
     scores(next_kd, next);
     Oct<K> p[2];
 #pragma unroll
@@ -1179,6 +1182,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
         x.raw = u4{lo[0], lo[1], up[0], up[1]};
         o[t] = mfma32(x.v, p[half].v, o[t]);
       }
+    __builtin_amdgcn_s_setprio(0);
   };
   // K runs one tile ahead of its use, V half a tile less: each load to LDS
   // has the time of a tile. Two barriers a tile: behind the first, K(kt + 1)
