@@ -1330,8 +1330,9 @@ int launch_join_by(Args& a, int tiles, int BM, int BN, int least,
 template <typename K, int D>
 int launch_join(Args& a, int tiles, int BM, int BN, int least,
                 hipStream_t stream) {
+  // many parts of few rows: several groups of lanes for a row
   const int parts = BN ? a.splits : a.workers / (tiles * a.Hk);
-  return parts >= 16
+  return parts >= 16 && tiles * a.Hk * BM <= 4096
              ? launch_join_by<K, D, 8>(a, tiles, BM, BN, least, stream)
              : launch_join_by<K, D, 1>(a, tiles, BM, BN, least, stream);
 }

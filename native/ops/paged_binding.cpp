@@ -298,18 +298,34 @@ struct Plan {
 // rows (new tokens * G) a sequence are work for the kernel for few rows, whose
 // `workers` share it out among themselves; 0 workers: the kernel for many
 // rows, with the keys of each tile of 128 rows in `splits` parts.
-Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t keys) {
+//
+// Splits: a workgroup by itself takes 1.3 us for 64 keys, so s parts save
+// 1.3 us * tiles * (1 - 1/s); they cost 4 us for the joining kernel and the
+// way of their sums through memory, at 4 TB/s, there and back. Measured (us,
+// unsplit against split): 184 rows on 272 keys 11.0/13.9, 251 tokens of 64
+// heads on 288 keys 14.7/20.2, 40 tokens of 32 heads on 688 keys 20.2/13.7,
+// 65 tokens of 32 heads on 4032 keys 109/32.5. Two workgroups fit a unit;
+// half more than that balance uneven sequences (295 rows a sequence on up to
+// 2368 keys: 2 parts 56.2, 3 parts 50.8), unless their tiles are mostly empty
+// and memory is what they wait for (22 rows: 5 parts 32.5, 8 parts 37.2).
+Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
+             int64_t keys) {
   const int64_t rows = T * G;
   // of keys that are worth a workgroup
   const int64_t pieces = std::max<int64_t>(1, (keys + 255) / 256);
   if (rows <= 16 * B) {
-    // two workgroups fit a unit; neighbouring ones share an XCD of eight
+    // neighbouring workgroups share an XCD of eight
     const int64_t items = Hk * std::max(B, rows / 16);
     const int64_t workers = std::min<int64_t>(512, items * pieces);
     return {(workers + 7) / 8 * 8, keys > 384, 1};  // 384: never split
   }
   const int64_t busy = Hk * std::max(B, rows / 128);
-  return {0, 0, std::min(pieces, std::max<int64_t>(1, 512 / busy))};
+  const int64_t splits =
+      std::min(pieces, (rows >= 64 * B ? 768 : 512) / busy);
+  if (splits <= 1) return {0, 0, 1};
+  const double saved = 1.3 * keys / 64 * (1 - 1.0 / splits);
+  const double spent = 4 + (double)rows * Hk * splits * D * 8 / 4e6;
+  return {0, 0, saved > spent ? splits : 1};
 }
 
 Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
@@ -354,7 +370,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
   if (T == 0 || B == 0) return out;
   const c10::DeviceGuard guard(p.device);
   q = rows_of(q);
-  const Plan plan = plan_of(T, B, G, Hk, cols << p.page_log2);
+  const Plan plan = plan_of(T, B, G, Hk, D, cols << p.page_log2);
   Tensor parts;
   if (plan.join || plan.splits > 1) {
     // its own for every call: two captured graphs never share it
@@ -501,10 +517,10 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    count(n, 5);
+    count(n, 6);
     const Plan p = plan_of(int_of(a[0], "T"), int_of(a[1], "B"),
                            int_of(a[2], "G"), int_of(a[3], "Hk"),
-                           int_of(a[4], "keys"));
+                           int_of(a[4], "D"), int_of(a[5], "keys"));
     return Py_BuildValue("LLL", (long long)p.workers, (long long)p.join,
                          (long long)p.splits);
   });

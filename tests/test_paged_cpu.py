@@ -152,7 +152,7 @@ def test_attention_refusals():
 def test_plan_covers_every_row(T, B, G):
     """Whatever the lengths, each sequence's tiles fit the grid."""
 
-    workers, join, splits = paged._ext().plan(T, B, G, 8, 4096)
+    workers, join, splits = paged._ext().plan(T, B, G, 8, 128, 4096)
     assert 1 <= splits <= 16
     assert workers == 0 or (join and 8 <= workers <= 512
                             and workers % 8 == 0)
