@@ -59,6 +59,7 @@ struct Args {
   long long q_row, q_head, table_row;
   int cols;  // of the table
   int T, B, Hq, Hk, G, pages, page_log2;
+  uint32_t inv_group;  // 2^32 / G, rounded up
   float scale;  // times log2(e): exponentials are of base 2
   int causal, splits;
   int workers;  // of the few kernel
@@ -70,15 +71,32 @@ struct Args {
 struct Span {
   int seq = -1;
   int row0, rows;  // the tile's first row, the sequence's rows
+  int t0, g0;      // of row0: its token, and head of the group
   int q0, n, len;  // first packed token, new tokens, keys
   bool broken;     // a length that the table cannot hold
 };
 
-// how many of the sequence's keys row r sees
-__device__ inline int seen_by(const Args& a, const Span& s, int r) {
-  if (r >= s.rows) return 0;
+// a row of a tile: its token of the sequence, and head of the kv head's group
+struct Row {
+  int t, g;
+};
+
+__device__ inline Row row_at(const Args& a, const Span& s, int i) {
+  // i and g0 are small: the product with 2^32 / G, rounded up, is exact
+  const int x = s.g0 + i;
+  const int q = a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.inv_group);
+  return Row{s.t0 + q, x - q * a.G};
+}
+
+// how many of the sequence's keys row i of the tile sees
+__device__ inline int seen_by(const Args& a, const Span& s, int i) {
+  if (s.row0 + i >= s.rows) return 0;
   if (!a.causal) return s.len;
-  return min(max(s.len - s.n + r / a.G + 1, 0), s.len);
+  return min(max(s.len - s.n + row_at(a, s, i).t + 1, 0), s.len);
+}
+// the last row's, of the first `rows`
+__device__ inline int most_seen(const Args& a, const Span& s, int rows) {
+  return seen_by(a, s, min(rows, s.rows - s.row0) - 1);
 }
 
 // tiles of keys: what this split takes of `all`, and how many splits work
@@ -305,8 +323,8 @@ __device__ inline Line line_of(const Args& a, Chunk& c, int BM) {
   l.head = __builtin_amdgcn_readlane(c.upto, 63);
   for (int base = 64; base < a.B; base += 64)
     l.head += __builtin_amdgcn_readlane(chunk_of(a, base, 0, BM).upto, 63);
-  l.per = max((int)(((long long)l.head * a.Hk + a.workers - 1) / a.workers),
-              NEAR);
+  l.per = max((int)((uint32_t)(l.head * a.Hk + a.workers - 1) /
+                    (uint32_t)a.workers), NEAR);
   return l;
 }
 
@@ -322,7 +340,7 @@ __device__ inline Item item_at(const Args& a, Chunk& c, int at, int BM) {
       r.units = __builtin_amdgcn_readlane(c.one, l);
       const int start = c.before + __builtin_amdgcn_readlane(c.upto, l) -
                         __builtin_amdgcn_readlane(c.own, l);
-      r.tile = (at - start) / r.units;
+      r.tile = at == start ? 0 : (at - start) / r.units;
       r.first = start + r.tile * r.units;
       return r;
     }
@@ -332,18 +350,6 @@ __device__ inline Item item_at(const Args& a, Chunk& c, int at, int BM) {
   }
 }
 
-// where worker w starts
-__device__ inline long long edge(const Args& a, const Line& l, Chunk& c,
-                                 int w, int BM) {
-  const long long at = (long long)w * l.per;
-  if (at >= (long long)l.head * a.Hk) return (long long)l.head * a.Hk;
-  const int h = (int)((uint32_t)at / (uint32_t)l.head);
-  const Item it = item_at(a, c, (int)(at - (long long)h * l.head), BM);
-  const long long first = (long long)h * l.head + it.first;
-  if (at - first < NEAR) return first;
-  return first + it.units - at < NEAR ? first + it.units : at;
-}
-
 // where the parts of an item that starts at unit `first` of the whole line
 // lie: part 0, and part i + 1 `stride` after part i from the second on
 struct Parts {
@@ -351,7 +357,7 @@ struct Parts {
   int count, stride;
 };
 
-__device__ inline Parts parts_of(const Line& l, long long first, int units) {
+__device__ inline Parts parts_of(const Line& l, int first, int units) {
   Parts p{0, 0, 1, 2};
   if (units < 2 * NEAR) return p;
   // the edges inside of the item
@@ -373,6 +379,8 @@ __device__ inline Span span_of(const Args& a, const Chunk& c, int seq,
   s.n = __builtin_amdgcn_readlane(c.n, l);
   s.rows = s.n * a.G;
   s.row0 = row0;
+  s.t0 = row0 ? row0 / a.G : 0;
+  s.g0 = row0 - s.t0 * a.G;
   s.len = __builtin_amdgcn_readlane(c.len, l);
   s.broken = s.len < 0;
   s.len = max(s.len, 0);
@@ -420,8 +428,8 @@ __device__ inline void join_rows(const Args& a, const Span& s, int h,
   __shared__ f4 sums[GS > 1 ? GROUPS : 1][LANES];
   __shared__ f2 tops[GROUPS];
   const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  const int row = row0 + group / GS, r = s.row0 + row;
-  const bool real = row < BM && r < s.rows;
+  const int row = row0 + group / GS;
+  const bool real = row < BM && s.row0 + row < s.rows;
 
   // parts group % GS, + GS, ...: 4 loads on their way at a time
   f4 x = {0, 0, 0, 0};
@@ -468,10 +476,11 @@ __device__ inline void join_rows(const Args& a, const Span& s, int h,
     }
   }
   if (!real) return;
-  const bool none = seen_by(a, s, r) == 0;
+  const bool none = seen_by(a, s, row) == 0;
   const float inv = s.broken ? nan_f32() : 1.0f / total;
-  T* dst = (T*)a.out + ((long long)(s.q0 + r / a.G) * a.Hq + h * a.G +
-                        r % a.G) * D + lane * 2;
+  const Row at = row_at(a, s, row);
+  T* dst = (T*)a.out +
+           ((long long)(s.q0 + at.t) * a.Hq + h * a.G + at.g) * D + lane * 2;
 #pragma unroll
   for (int j = 0; j < 4; j += 2) {
     const T y[2] = {none && !s.broken ? (T)0.0f : (T)(x[j] * inv),
@@ -514,19 +523,16 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   asm volatile("" : "+v"(lane));
   const int col = lane & 15, grp = lane >> 4;
 
-  const int seen_min = seen_by(a, s, s.row0);
-  const int last_row = min(s.row0 + BM, s.rows) - 1;
-  const int seen_max = seen_by(a, s, last_row);
+  const int seen_min = seen_by(a, s, 0), seen_max = most_seen(a, s, BM);
 
   // Q: a lane holds 8 values of row `col` for each step
   Oct<K> q[NF];
-  const int seen = seen_by(a, s, s.row0 + col);
+  const int seen = seen_by(a, s, col);
   {
-    const int r = s.row0 + col;
-    const bool real = r < s.rows;
-    const int t = real ? r / a.G : 0, g = real ? r % a.G : 0;
-    const T* src = (const T*)a.q + (s.q0 + t) * a.q_row +
-                   (long long)(h * a.G + g) * a.q_head;
+    const bool real = s.row0 + col < s.rows;
+    const Row r = row_at(a, s, real ? col : 0);
+    const T* src = (const T*)a.q + (s.q0 + r.t) * a.q_row +
+                   (long long)(h * a.G + r.g) * a.q_head;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const int d0 = KB == 16 && Q8 ? 64 * (f >> 1) + grp * 16 + (f & 1) * 8
@@ -559,17 +565,17 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   const uint32_t k_off = col * (D * EB) + grp * KB;
   const uint32_t v_off = lane * 16;
 
-  auto fetch = [&](Arrival& to, int kt) {
-    const bool bad0 = to.bad0 = (unsigned)id[0] >= (unsigned)a.pages;
-    const bool bad1 = to.bad1 = (unsigned)id[1] >= (unsigned)a.pages;
-    const int key = kt * BN;
-    const long long row0 = (((long long)(bad0 ? 0 : id[0]) * a.Hk + h)
-                            << a.page_log2) + (key & in_page);
-    const long long row1 = (((long long)(bad1 ? 0 : id[1]) * a.Hk + h)
-                            << a.page_log2) + ((key + 16) & in_page);
+  auto row_of = [&](int id, int key) {
+    const bool bad = (unsigned)id >= (unsigned)a.pages;
+    return (((long long)(bad ? 0 : id) * a.Hk + h) << a.page_log2) +
+           (key & in_page);
+  };
+  auto fetch_k = [&](Arrival& to, int kt) {
+    to.bad0 = (unsigned)id[0] >= (unsigned)a.pages;
+    to.bad1 = (unsigned)id[1] >= (unsigned)a.pages;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const long long row = half ? row1 : row0;
+      const long long row = row_of(id[half], kt * BN + half * 16);
       const uint8_t* src = kc + row * (D * EB);
       if constexpr (Q8) to.ksr[half] = (a.k_scale + row)[col];
 #pragma unroll
@@ -582,6 +588,10 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
         }
       }
     }
+  };
+  auto fetch_v = [&](Arrival& to, int kt) {
+    const long long row0 = row_of(id[0], kt * BN);
+    const long long row1 = row_of(id[1], kt * BN + 16);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if constexpr (VROWS <= 16) {
@@ -622,19 +632,27 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   if (kt < mine.last) {
     id[0] = page_of(kt * BN);
     id[1] = page_of(kt * BN + 16);
-    fetch(arrivals[0], kt);
+    fetch_k(arrivals[0], kt);
+    fetch_v(arrivals[0], kt);
     id[0] = page_of((kt + WAVES) * BN);
     id[1] = page_of((kt + WAVES) * BN + 16);
   }
-  auto fetch_next = [&](Arrival& to) {
+  auto next_k = [&](Arrival& to) {
+    if (kt + WAVES < mine.last) fetch_k(to, kt + WAVES);
+  };
+  auto next_v = [&](Arrival& to) {
     if (kt + WAVES < mine.last) {
-      fetch(to, kt + WAVES);
+      fetch_v(to, kt + WAVES);
       id[0] = page_of((kt + 2 * WAVES) * BN);
       id[1] = page_of((kt + 2 * WAVES) * BN + 16);
     }
   };
+  // The next tile's loads start as soon as there are registers for them.
   auto take = [&](Arrival& now, Arrival& next) {
-    if constexpr (AHEAD) fetch_next(next);
+    if constexpr (AHEAD) {
+      next_k(next);
+      next_v(next);
+    }
     const int key0 = kt * BN;
     const bool none0 = now.bad0, none1 = now.bad1;
 
@@ -658,6 +676,8 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
         sc[half] = mfma16(x.v, q[f].v, sc[half]);
       }
     }
+
+    if constexpr (!AHEAD) next_k(next);
 
     // V to the wave's LDS; rows past the end, or without a page, as 0
     const bool past = key0 + BN > seen_max || none0 || none1;
@@ -693,8 +713,7 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
     }
     wave_fence();
 
-    // the next tile is on its way while this one's softmax is worked out
-    if constexpr (!AHEAD) fetch_next(next);
+    if constexpr (!AHEAD) next_v(next);
 
     Oct<K> p;
     if (cut) {
@@ -786,8 +805,8 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   for (int t = 0; t < NT; ++t)
     *reinterpret_cast<f4*>(&all[wave][col][t * 16 + grp * 4]) = o[t];
   __syncthreads();
-  const int row = threadIdx.x >> 4, r = s.row0 + row;
-  if (r >= s.rows) return;
+  const int row = threadIdx.x >> 4;
+  if (s.row0 + row >= s.rows) return;
   float top = minus_inf();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[0][w][row]);
@@ -800,10 +819,10 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   }
   // pairs of values, 16 lanes a row: stores of one run of memory
   const int d0 = (threadIdx.x & 15) * 2;
-  const int t = r / a.G, g = r % a.G;
-  const bool none = seen_by(a, s, r) == 0;
+  const Row r = row_at(a, s, row);
+  const bool none = seen_by(a, s, row) == 0;
   const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
-  T* dst = (T*)a.out + ((long long)(s.q0 + t) * a.Hq + h * a.G + g) * D;
+  T* dst = (T*)a.out + ((long long)(s.q0 + r.t) * a.Hq + h * a.G + r.g) * D;
   const long long at = part * BM + row;
 #pragma unroll
   for (int d = d0; d < D; d += 32) {
@@ -842,26 +861,50 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
   const int w = a.workers % 8 ? blockIdx.x
                               : blockIdx.x % 8 * (a.workers / 8) +
                                     blockIdx.x / 8;
-  long long at = edge(a, line, c, w, BM);
-  const long long end = edge(a, line, c, w + 1, BM);
-  while (at < end) {
-    const int h = (int)((uint32_t)at / (uint32_t)line.head);
-    const long long start = (long long)h * line.head;
-    const Item it = item_at(a, c, (int)(at - start), BM);
-    if (it.seq < 0) return;
+  const int total = line.head * a.Hk;
+  int end = w * line.per;
+  if (end >= total) return;
+  int h = (int)((uint32_t)end / (uint32_t)line.head);
+  Item it = item_at(a, c, end - h * line.head, BM);
+  if (it.seq < 0) return;
+  int from = end - h * line.head - it.first;
+  end += line.per;
+  bool next = false;
+  if (from < NEAR)
+    from = 0;
+  else if (it.units - from < NEAR)
+    next = true;
+  while (true) {
+    if (next) {
+      int at = it.first + it.units;
+      if (at == line.head) {
+        at = 0;
+        if (++h == a.Hk) return;
+      }
+      it = item_at(a, c, at, BM);
+      if (it.seq < 0) return;
+      from = 0;
+    }
+    // the next worker's edge, if it is in this item
+    int to = it.units;
+    if (end < total) {
+      const int e = end - h * line.head - it.first;
+      if (e < it.units) {
+        if (e < NEAR) return;
+        if (it.units - e >= NEAR) to = e;
+      }
+    }
     const Span s = span_of(a, c, it.seq, it.tile * BM);
-    const int from = (int)(at - start) - it.first;
-    const int to = (int)min((long long)it.units, from + (end - at));
     // an item's last units may hold no key that its rows see
-    const int all =
-        (seen_by(a, s, min(s.row0 + BM, s.rows) - 1) + BN - 1) / BN;
+    const int all = (most_seen(a, s, BM) + BN - 1) / BN;
     Share mine;
     mine.first = min(max(from - OWN, 0) << a.unit_log2, all);
     mine.last = min(max(to - OWN, 0) << a.unit_log2, all);
-    const bool whole = from == 0 && to == it.units;
-    few_part<K, D, Q8>(a, lds, stat, s, h, mine, whole,
-                           2LL * w + (from == 0 ? 1 : 0));
-    at += to - from;
+    few_part<K, D, Q8>(a, lds, stat, s, h, mine,
+                       from == 0 && to == it.units,
+                       2LL * w + (from == 0 ? 1 : 0));
+    if (to < it.units) return;
+    next = true;
     __syncthreads();
   }
 }
@@ -926,8 +969,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   const int lane = threadIdx.x & 63;
   const int col = lane & 31, hi = lane >> 5;
 
-  const int seen_min = seen_by(a, s, s.row0);
-  const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
+  const int seen_min = seen_by(a, s, 0), seen_max = most_seen(a, s, BM);
   const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
                               4);
   if ((int)blockIdx.y >= mine.active) return;
@@ -935,18 +977,17 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   __syncthreads();
 
   // this wave's rows
-  const int w0 = s.row0 + wave * 32, r = w0 + col;
-  const bool real = r < s.rows;
-  const int my_t = real ? r / a.G : 0, my_g = real ? r % a.G : 0;
-  const int seen = seen_by(a, s, r);
-  const int wave_min =
-      w0 + 31 < s.rows ? seen_by(a, s, w0) : 0;  // rows past the end see none
-  const int wave_max =
-      w0 < s.rows ? seen_by(a, s, min(w0 + 32, s.rows) - 1) : 0;
+  const int w0 = wave * 32;
+  const bool real = s.row0 + w0 + col < s.rows;
+  const Row my = row_at(a, s, real ? w0 + col : 0);
+  const int seen = seen_by(a, s, w0 + col);
+  const bool full = s.row0 + w0 + 31 < s.rows;
+  const int wave_min = full ? seen_by(a, s, w0) : 0;  // past the end: none
+  const int wave_max = s.row0 + w0 < s.rows ? most_seen(a, s, w0 + 32) : 0;
   Oct<K> q[NF];
   {
-    const T* src = (const T*)a.q + (s.q0 + my_t) * a.q_row +
-                   (long long)(h * a.G + my_g) * a.q_head;
+    const T* src = (const T*)a.q + (s.q0 + my.t) * a.q_row +
+                   (long long)(h * a.G + my.g) * a.q_head;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       q[f].raw = real ? *reinterpret_cast<const u4*>(src + f * 16 + hi * 8)
@@ -1260,7 +1301,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
     const bool none = seen == 0;
     const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / sum;
     T* dst = (T*)a.out +
-             ((long long)(s.q0 + my_t) * a.Hq + h * a.G + my_g) * D;
+             ((long long)(s.q0 + my.t) * a.Hq + h * a.G + my.g) * D;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -1298,15 +1339,15 @@ join_kernel(Args a, int BM, int BN, int least) {
   if (s.seq < 0) return;
   Parts p;
   if (BN) {
-    const int seen_max = seen_by(a, s, min(s.row0 + BM, s.rows) - 1);
-    p.count = share_of((seen_max + BN - 1) / BN, a.splits, 0, least).active;
+    p.count = share_of((most_seen(a, s, BM) + BN - 1) / BN, a.splits, 0,
+                       least).active;
     p.part0 = (long long)blockIdx.x * a.splits;
     p.part1 = p.part0 + 1;
     p.stride = 1;
   } else {
     const int l = s.seq - c.base;
     const int units = __builtin_amdgcn_readlane(c.one, l);
-    p = parts_of(line, (long long)h * line.head + c.before +
+    p = parts_of(line, h * line.head + c.before +
                            __builtin_amdgcn_readlane(c.upto, l) -
                            __builtin_amdgcn_readlane(c.own, l) +
                            s.row0 / BM * units, units);
@@ -1391,7 +1432,7 @@ int tf_paged_attention(
     int Hk, int pages, int page_log2, int D, float scale, int causal,
     int fp16, int workers, int join, int splits,
     void* stream) {
-  if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || cols < 0 ||
+  if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || Hq > 32768 || cols < 0 ||
       pages < 1 || page_log2 < 4 || page_log2 > 10 ||
       workers < 0 || splits < 1 || splits > 65535 ||
       (workers && !join && (cols << page_log2) > (2 * NEAR - OWN) * 32) ||
@@ -1403,6 +1444,7 @@ int tf_paged_attention(
          (const int*)q_starts, (const int*)kv_lens, (const int*)table, out,
          (float*)parts, nullptr, q_row, q_head, table_row, cols, T, B, Hq, Hk,
          Hq / Hk, pages, page_log2,
+         (uint32_t)(((1ULL << 32) + Hq / Hk - 1) / (Hq / Hk)),
          // 0 times a masked score would be NaN; this leaves every p 1 too
          scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 1, 0};
   // a line of less than 2^30 units, as bounded by what the host knows

@@ -353,7 +353,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
     refuse(cols, " pages of ", 1 << p.page_log2, " tokens: a sequence has at "
            "most 2**30");
   const int64_t G = Hq / Hk, most = 1LL << 31;
-  if (T >= most || B >= most || T * G + 128 * B >= most ||
+  if (Hq > 32768 || T >= most || B >= most || T * G + 128 * B >= most ||
       (T * G / 16 + B) * Hk >= most)
     refuse(T, " tokens of ", Hq, " heads: too many for a launch");
   if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)D);
