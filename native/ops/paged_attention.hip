@@ -267,12 +267,20 @@ __device__ inline void wave_fence() {
 // The work is one line: for each kv head, each sequence, each of its tiles of
 // rows, an item of OWN + (its keys / unit keys) units. Worker w takes the
 // units from edge(w) to edge(w + 1): w * per, moved to an item's start or end
-// where that is less than NEAR away. So workers end together however ragged
-// the batch is, items of up to 2 NEAR units are never split, and of a
-// worker's items at most two are split: one that it starts (its part is in
+// where that is less than near(item) away. So workers end together however
+// ragged the batch is, items of less than WHOLE units are never split, and of
+// a worker's items at most two are split: one that it starts (its part is in
 // place 1), and one that it goes on with (place 0). A unit is 32 keys, or
 // more where the line would pass 2^30 units.
-constexpr int OWN = 4, NEAR = 8;
+//
+// WHOLE: a workgroup takes 128 keys in 1.1 us, and the kernel that joins two
+// parts takes 4 us; 8 sequences of 560 keys and 8 heads: in two parts 14.8 us,
+// whole 11.6 us.
+constexpr int OWN = 4, NEAR = 4, LEAST = 8, WHOLE = 32;
+
+__device__ inline int near(int units) {
+  return units < WHOLE ? units / 2 + 1 : NEAR;
+}
 
 struct Item {
   int seq, tile;  // tile of the sequence's rows
@@ -324,7 +332,7 @@ __device__ inline Line line_of(const Args& a, Chunk& c, int BM) {
   for (int base = 64; base < a.B; base += 64)
     l.head += __builtin_amdgcn_readlane(chunk_of(a, base, 0, BM).upto, 63);
   l.per = max((int)((uint32_t)(l.head * a.Hk + a.workers - 1) /
-                    (uint32_t)a.workers), NEAR);
+                    (uint32_t)a.workers), LEAST);
   return l;
 }
 
@@ -359,7 +367,7 @@ struct Parts {
 
 __device__ inline Parts parts_of(const Line& l, int first, int units) {
   Parts p{0, 0, 1, 2};
-  if (units < 2 * NEAR) return p;
+  if (units < WHOLE) return p;
   // the edges inside of the item
   const int w0 = (int)((uint32_t)(first + NEAR + l.per - 1) / (uint32_t)l.per);
   const int w1 = (int)((uint32_t)(first + units - NEAR) / (uint32_t)l.per);
@@ -870,9 +878,9 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
   int from = end - h * line.head - it.first;
   end += line.per;
   bool next = false;
-  if (from < NEAR)
+  if (from < near(it.units))
     from = 0;
-  else if (it.units - from < NEAR)
+  else if (it.units - from < near(it.units))
     next = true;
   while (true) {
     if (next) {
@@ -890,8 +898,8 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
     if (end < total) {
       const int e = end - h * line.head - it.first;
       if (e < it.units) {
-        if (e < NEAR) return;
-        if (it.units - e >= NEAR) to = e;
+        if (e < near(it.units)) return;
+        if (it.units - e >= near(it.units)) to = e;
       }
     }
     const Span s = span_of(a, c, it.seq, it.tile * BM);
@@ -1435,7 +1443,7 @@ int tf_paged_attention(
   if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || Hq > 32768 || cols < 0 ||
       pages < 1 || page_log2 < 4 || page_log2 > 10 ||
       workers < 0 || splits < 1 || splits > 65535 ||
-      (workers && !join && (cols << page_log2) > (2 * NEAR - OWN) * 32) ||
+      (workers && !join && (cols << page_log2) > (WHOLE - 1 - OWN) * 32) ||
       ((join || splits > 1) && !parts) ||
       ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
       (long long)T * (Hq / Hk) + 128LL * B >= (1LL << 31))

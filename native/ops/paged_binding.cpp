@@ -317,7 +317,7 @@ Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
     // neighbouring workgroups share an XCD of eight
     const int64_t items = Hk * std::max(B, rows / 16);
     const int64_t workers = std::min<int64_t>(512, items * pieces);
-    return {(workers + 7) / 8 * 8, keys > 384, 1};  // 384: never split
+    return {(workers + 7) / 8 * 8, keys > 864, 1};  // 864: never split
   }
   const int64_t busy = Hk * std::max(B, rows / 128);
   const int64_t splits =

@@ -93,6 +93,23 @@ def apply_rope(x, cos, sin, pos):
     return out
 
 
+def is_paged(cache) -> bool:
+    """Whether a layer's cache is (PagedKVCache, PagedBatch), as
+    PagedBatch.over gives it."""
+
+    if cache is None or isinstance(cache[0], torch.Tensor):
+        return False
+    from ..ops import paged
+    return isinstance(cache[0], paged.PagedKVCache)
+
+
+def paged_caches(layers: int, pages: int, page_size: int, kv_heads: int,
+                 head_dim: int, device, dtype, quantized: bool):
+    from ..ops import paged
+    return [paged.make_cache(pages, page_size, kv_heads, head_dim, dtype,
+                             quantized, device) for _ in range(layers)]
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
@@ -129,10 +146,37 @@ class Attention(nn.Module):
             flat = flat.contiguous()
         return fused.skinny_gemm_packed(flat, wp, lin.out_features)             .view(B, T, -1)
 
+    def _merged_qkv(self, x):
+        """q, k and v as columns of ONE product (decode is weight
+        streaming: 3 launches -> 1)."""
+
+        if self._wqkv is None:
+            self._wqkv = torch.cat(
+                [self.wq.weight, self.wk.weight, self.wv.weight],
+                dim=0).detach().contiguous()
+        dk = self.cfg.kv_heads * self.head_dim
+        return F.linear(x, self._wqkv).split(
+            [self.cfg.heads * self.head_dim, dk, dk], dim=-1)
+
+    def _paged(self, x, cos, sin, cache, batch):
+        """Rotation, cache write and attention over pages: two kernels of
+        ops/paged.py, for new tokens of any number of sequences."""
+
+        from ..ops import paged
+        if _FUSED_OPS:
+            q, k, v = self._merged_qkv(x)
+        else:
+            q, k, v = self.wq(x), self.wk(x), self.wv(x)
+        o = paged.attend(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1),
+                         cos, sin, cache, batch, self.cfg.heads)
+        return self._proj(self.wo, o.view(*x.shape[:2], -1), 3)
+
     def forward(self, x, cos, sin, pos, cache=None, pos_end=None,
                 mask=None):
         B, T, _ = x.shape
         cfg = self.cfg
+        if is_paged(cache):
+            return self._paged(x, cos, sin, *cache)
         if (_FUSED_OPS and x.is_cuda and x.dtype == torch.bfloat16
                 and cache is not None and self.head_dim % 8 == 0
                 and isinstance(pos, torch.Tensor) and cos.is_contiguous()):
@@ -142,16 +186,7 @@ class Attention(nn.Module):
             # launches -> 1; the rope kernel reads the column slices
             # with their row stride)
             from ..ops import fused
-            if self._wqkv is None:
-                self._wqkv = torch.cat(
-                    [self.wq.weight, self.wk.weight, self.wv.weight],
-                    dim=0).detach().contiguous()
-            qkv = F.linear(x, self._wqkv)
-            dq = cfg.heads * self.head_dim
-            dk = cfg.kv_heads * self.head_dim
-            qin = qkv[..., :dq]
-            kin = qkv[..., dq:dq + dk]
-            vin = qkv[..., dq + dk:]
+            qin, kin, vin = self._merged_qkv(x)
             k_cache, v_cache = cache
             q = fused.rope_qkv_cache(qin, kin, vin, cos, sin, pos,
                                      k_cache, v_cache, cfg.heads,
@@ -332,6 +367,22 @@ class Llama(nn.Module):
                              dtype=dtype)) for _ in range(cfg.layers)]
 
 
+    def make_paged_cache(self, pages: int, page_size: int, device, dtype,
+                         quantized: bool = False):
+        """One paged cache a layer (ops/paged.py). A forward pass over it
+        takes a PagedBatch's positions and layers:
+
+            batch = PagedBatch.of(block_table, past, new, page_size)
+            model(tokens, pos=batch.pos, caches=batch.over(caches))
+
+        with tokens [B, new], or [1, all] for sequences of different new
+        lengths; no mask, and no `pos_end`. Under torch.no_grad()."""
+
+        cfg = self.cfg
+        return paged_caches(cfg.layers, pages, page_size, cfg.kv_heads,
+                            cfg.dim // cfg.heads, device, dtype, quantized)
+
+
 @torch.no_grad()
 def build_model(name: str, device="cuda", dtype=torch.bfloat16,
                 seed: int = 0) -> Llama:
@@ -438,6 +489,61 @@ def decode_bench_graphs(model: Llama, batch: int, ctx: int, steps: int,
     return batch * steps / dt, dt / steps * 1000.0
 
 
+@torch.no_grad()
+def decode_bench_paged(model: Llama, batch: int, ctx: int, steps: int,
+                       warmup: int, page_size: int = 64,
+                       quantized: bool = False, graphs: bool = False,
+                       device="cuda", dtype=torch.bfloat16):
+    """decode_bench over a paged cache, eager or as one captured graph a
+    step: positions, slots and lengths advance on the device, and attention
+    reads the valid keys only."""
+
+    from ..ops.paged import PagedBatch
+    cfg = model.cfg
+    warmup = max(warmup, 1)
+    width = -(-(ctx + steps + warmup + 8) // page_size)
+    caches = model.make_paged_cache(batch * width, page_size, device, dtype,
+                                    quantized)
+    table = torch.arange(batch * width, device=device,
+                         dtype=torch.int32).view(batch, width)
+    past = torch.zeros(batch, dtype=torch.int64, device=device)
+    toks = torch.randint(0, cfg.vocab, (batch, ctx), device=device)
+    first = PagedBatch.of(table, past, ctx, page_size)
+    model(toks, pos=first.pos, caches=first.over(caches))
+    past.add_(ctx)
+    cur = torch.randint(0, cfg.vocab, (batch, 1), device=device)
+
+    def step():
+        b = PagedBatch.of(table, past, 1, page_size)
+        logits = model(cur, pos=b.pos, caches=b.over(caches))
+        cur.copy_(logits.argmax(-1))
+        past.add_(1)
+
+    if graphs:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        run = g.replay
+    else:
+        run = step
+    for _ in range(warmup):
+        run()
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    for _ in range(steps):
+        run()
+    torch.cuda.synchronize()
+    dt = time.perf_counter() - t0
+    return batch * steps / dt, dt / steps * 1000.0
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", default="llama3-8b")
@@ -449,11 +555,23 @@ def main():
     ap.add_argument("--dtype", default="bf16")
     ap.add_argument("--graphs", action="store_true",
                     help="hipGraph-captured decode loop")
+    ap.add_argument("--paged", action="store_true",
+                    help="paged KV cache and its attention (ops/paged.py)")
+    ap.add_argument("--page-size", type=int, default=64)
+    ap.add_argument("--kv-e4m3", action="store_true",
+                    help="keep the paged cache in 8 bits")
     args = ap.parse_args()
     dtype = {"bf16": torch.bfloat16, "fp16": torch.float16,
              "fp32": torch.float32}[args.dtype]
     model = build_model(args.model, device=args.device, dtype=dtype)
-    if args.graphs or os.environ.get("TF_BENCH_GRAPHS") == "1":
+    graphs = args.graphs or os.environ.get("TF_BENCH_GRAPHS") == "1"
+    if args.kv_e4m3 and not args.paged:
+        ap.error("--kv-e4m3 is for a --paged cache")
+    if args.paged:
+        tok_s, ms = decode_bench_paged(
+            model, args.batch, args.ctx, args.steps, args.warmup,
+            args.page_size, args.kv_e4m3, graphs, args.device, dtype)
+    elif graphs:
         tok_s, ms = decode_bench_graphs(model, args.batch, args.ctx,
                                         args.steps, args.warmup,
                                         device=args.device, dtype=dtype)

@@ -27,6 +27,7 @@ from __future__ import annotations
 import importlib.machinery
 import importlib.util
 import os
+from dataclasses import dataclass
 
 import torch
 
@@ -112,6 +113,74 @@ def make_cache(pages: int, page_size: int, kv_heads: int, head_dim: int,
         return PagedKVCache(k, v, ks, vs)
     return PagedKVCache(torch.zeros(shape, dtype=dtype, device=device),
                         torch.zeros(shape, dtype=dtype, device=device))
+
+
+@dataclass
+class PagedBatch:
+    """New tokens of some sequences, as the operators take them: packed one
+    sequence after the other, token i at position pos[i] of its sequence, in
+    slot slots[i]; kv_lens counts them."""
+
+    q_starts: torch.Tensor      # int32 [B + 1]
+    kv_lens: torch.Tensor       # int32 [B]
+    block_table: torch.Tensor   # int32 [B, columns]
+    pos: torch.Tensor           # int64 [tokens]
+    slots: torch.Tensor         # int64 [tokens]
+
+    @classmethod
+    def of(cls, block_table, past, new, page_size: int) -> "PagedBatch":
+        """`new` tokens (a number, or one for each sequence) behind the
+        first `past` (integers [B]) of the sequences of a block table. With
+        a number everything is worked out on the device, so that a step that
+        is captured goes on from wherever `past` stands at the replay."""
+
+        (B, cols), device = block_table.shape, block_table.device
+        past = past.to(torch.int64)
+        if isinstance(new, int):
+            starts = torch.arange(B + 1, device=device,
+                                  dtype=torch.int32) * new
+            pos = past[:, None] + torch.arange(new, device=device)
+            seq = torch.arange(B, device=device)[:, None].expand(B, new)
+            pos, seq, lens = pos.flatten(), seq.flatten(), past + new
+        else:
+            if len(new) != B or min(new, default=0) < 0:
+                raise ValueError(f"{len(new)} counts {list(new)[:8]} for {B} "
+                                 "sequences")
+            n = torch.tensor(new, dtype=torch.int64)
+            starts = torch.zeros(B + 1, dtype=torch.int64)
+            starts[1:] = n.cumsum(0)
+            seq = torch.arange(B).repeat_interleave(n)
+            pos = torch.arange(len(seq)) - starts[seq]
+            seq = seq.to(device)
+            pos = pos.to(device) + past[seq]
+            lens = past + n.to(device)
+            starts = starts.to(torch.int32).to(device)
+        if cols == 0 and len(pos):
+            raise ValueError("a block table without columns has no slots")
+        # a position that the table does not hold has no slot
+        col = pos // page_size
+        there = (pos >= 0) & (col < cols)
+        page = block_table[seq, col.clamp(0, max(cols - 1, 0))]
+        slots = page.to(torch.int64) * page_size + pos % page_size
+        slots = torch.where(there, slots, -1)
+        return cls(starts, lens.to(torch.int32), block_table, pos, slots)
+
+    def over(self, caches):
+        """The layers' caches, as a model takes them with this batch."""
+
+        return [(c, self) for c in caches]
+
+
+def attend(q_in, k_in, v_in, cos, sin, cache: PagedKVCache,
+           batch: PagedBatch, heads: int):
+    """A layer's attention between its projections: rope_kv_write, then
+    paged_attention. Returns [tokens, heads * head_dim]."""
+
+    q = rope_kv_write(cache, q_in, k_in, v_in, cos, sin, batch.pos,
+                      batch.slots, heads)
+    out = paged_attention(q, cache, batch.q_starts, batch.kv_lens,
+                          batch.block_table)
+    return out.flatten(1)
 
 
 def kv_write(cache: PagedKVCache, k, v, slots) -> None:

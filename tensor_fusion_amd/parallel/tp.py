@@ -26,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..models.llama import (CONFIGS, Llama, LlamaConfig, RMSNorm,
-                            apply_rope)
+                            apply_rope, is_paged, paged_caches)
 
 
 def _world():
@@ -85,6 +85,12 @@ class TPAttention(nn.Module):
     def forward(self, x, cos, sin, pos, cache=None, pos_end=None,
                 mask=None):
         B, T, _ = x.shape
+        if is_paged(cache):
+            from ..ops import paged
+            o = paged.attend(*(w(x).flatten(0, 1) for w in (self.wq, self.wk,
+                                                            self.wv)),
+                             cos, sin, *cache, self.heads)
+            return self.wo(o.view(B, T, -1))
         q = self.wq(x).view(B, T, self.heads, self.head_dim).transpose(1, 2)
         k = self.wk(x).view(B, T, self.kv_heads, self.head_dim).transpose(1, 2)
         v = self.wv(x).view(B, T, self.kv_heads, self.head_dim).transpose(1, 2)
@@ -165,6 +171,17 @@ class TPLlama(nn.Module):
                              dtype=dtype),
                  torch.zeros(batch, kv, max_seq, hd, device=device,
                              dtype=dtype)) for _ in range(cfg.layers)]
+
+
+    def make_paged_cache(self, pages: int, page_size: int, device, dtype,
+                         quantized: bool = False):
+        """Llama.make_paged_cache with this rank's heads; the block table
+        is every rank's."""
+
+        cfg = self.cfg
+        return paged_caches(cfg.layers, pages, page_size,
+                            cfg.kv_heads // self.tp, cfg.dim // cfg.heads,
+                            device, dtype, quantized)
 
 
 @torch.no_grad()
