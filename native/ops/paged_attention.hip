@@ -104,6 +104,9 @@ struct Share {
   int first, last, active;
 };
 
+// keys of a tile of the many kernel, and the fewest tiles of a split
+constexpr int MANY_KEYS = 64, MANY_LEAST = 4;
+
 __device__ inline Share share_of(int all, int splits, int split, int least) {
   int each = max((all + splits - 1) / splits, least);
   Share s;
@@ -398,29 +401,28 @@ __device__ inline Span span_of(const Args& a, const Chunk& c, int seq,
 // Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
 // leaves each at least its own number, needs no sum over the sequences
 // before it, and the last such start at or below `tile` is its sequence.
-__device__ inline Span find(const Args& a, Chunk& c, int tile, int BM) {
-  Span s;
-  while (true) {
-    const int lane = threadIdx.x & 63;
-    const int first = c.q0 * a.G / BM + c.base + lane;
-    const unsigned long long at =
-        __ballot(c.base + lane < a.B && first <= tile);
-    if (at == 0) return s;
-    const int last = 63 - __clzll(at);
-    // the next chunk's first sequence may start at or below the tile as well
-    if (last == 63 && c.base + 64 < a.B) {
-      const int q0 = min(max(a.q_starts[c.base + 64], 0), a.T);
-      if (q0 * a.G / BM + c.base + 64 <= tile) {
-        c = chunk_of(a, c.base + 64,
-                     c.before + __builtin_amdgcn_readlane(c.upto, 63), BM);
-        continue;
-      }
-    }
-    const Span r = span_of(
-        a, c, c.base + last,
-        (tile - __builtin_amdgcn_readlane(first, last)) * BM);
-    return r.row0 < r.rows ? r : s;
+__device__ inline Span find(const Args& a, int tile, int BM) {
+  // the last 64 sequences whose first one starts at or below the tile
+  int base = 0;
+  for (int above = (a.B + 63) / 64; above - base > 1;) {
+    const int mid = (base + above) / 2;
+    const int q0 = min(max(uniform_load(a.q_starts + mid * 64), 0), a.T);
+    if (q0 * a.G / BM + mid * 64 <= tile)
+      base = mid;
+    else
+      above = mid;
   }
+  const Chunk c = chunk_of(a, base * 64, 0, BM);
+  const int lane = threadIdx.x & 63;
+  const int first = c.q0 * a.G / BM + c.base + lane;
+  const unsigned long long at =
+      __ballot(c.base + lane < a.B && first <= tile);
+  if (at == 0) return Span();
+  const int last = 63 - __clzll(at);
+  const Span s =
+      span_of(a, c, c.base + last,
+              (tile - __builtin_amdgcn_readlane(first, last)) * BM);
+  return s.row0 < s.rows ? s : Span();
 }
 
 // ---- the splits' parts ------------------------------------------------------
@@ -955,7 +957,7 @@ __device__ inline uint32_t lds_address(const void* p) {
 template <typename K, int D, bool Q8>
 __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   typedef typename K::T T;
-  constexpr int BM = 128, BN = 64, WAVES = 4;
+  constexpr int BM = 128, BN = MANY_KEYS;
   constexpr int NF = D / 16;            // steps of the product over D
   constexpr int NT = D / 32;            // tiles of 32 values of O^T
   constexpr int EB = Q8 ? 1 : 2;
@@ -970,8 +972,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
-  Chunk c = chunk_of(a, 0, 0, BM);
-  const Span s = find(a, c, tile, BM);
+  const Span s = find(a, tile, BM);
   if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -979,7 +980,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 
   const int seen_min = seen_by(a, s, 0), seen_max = most_seen(a, s, BM);
   const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
-                              4);
+                              MANY_LEAST);
   if ((int)blockIdx.y >= mine.active) return;
   if (threadIdx.x == 0) odd_v = 0;
   __syncthreads();
@@ -1241,8 +1242,8 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   int id1 = page_of(kt), id2 = page_of(kt + 1);  // of the next V, the next K
   if (kt < mine.last) {
     fetch_k(id1, kt);
-    put_k(id1, kt, false);
     fetch_v(id1, kt);
+    put_k(id1, kt, true);
     put_v(id1, kt, false);
     if (kt + 1 < mine.last) fetch_k(id2, kt + 1);
   }
@@ -1333,57 +1334,83 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   }
 }
 
-// One workgroup for ROWS rows of a tile.
-// BN, least: what the many kernel shared its keys by; 0: the parts of the
-// few kernel.
+// Up to 4 workgroups for the rows of an item of the few kernel: that in which
+// worker w > 0 has its edge, if it is the first edge in it.
 template <typename K, int D, int GS>
-__global__ void __launch_bounds__(256)
-join_kernel(Args a, int BM, int BN, int least) {
-  constexpr int ROWS = 256 / (D / 4) / GS;
-  const int h = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
+__global__ void __launch_bounds__(256) join_few_kernel(Args a) {
+  constexpr int BM = 16, ROWS = 256 / (D / 4) / GS;
+  const int w = blockIdx.x + 1;
   Chunk c;
   const Line line = line_of(a, c, BM);
-  const Span s = find(a, c, tile, BM);
+  const int at = w * line.per;
+  if (at >= line.head * a.Hk) return;
+  const int h = (int)((uint32_t)at / (uint32_t)line.head);
+  const Item it = item_at(a, c, at - h * line.head, BM);
+  if (it.seq < 0 || it.units < WHOLE) return;
+  const int first = h * line.head + it.first;
+  if (at - first < NEAR || first + it.units - at < NEAR ||
+      at - line.per - first >= NEAR)
+    return;
+  const Span s = span_of(a, c, it.seq, it.tile * BM);
+  const Parts p = parts_of(line, first, it.units);
+  for (int row = blockIdx.y * ROWS; row < BM && s.row0 + row < s.rows;
+       row += gridDim.y * ROWS) {
+    join_rows<K, D, GS>(a, s, h, p, BM, row);
+    __syncthreads();
+  }
+}
+
+// One workgroup for ROWS rows of a tile of the many kernel.
+template <typename K, int D, int GS>
+__global__ void __launch_bounds__(256) join_many_kernel(Args a) {
+  constexpr int BM = 128, ROWS = 256 / (D / 4) / GS;
+  const Span s = find(a, blockIdx.x / a.Hk, BM);
   if (s.seq < 0) return;
   Parts p;
-  if (BN) {
-    p.count = share_of((most_seen(a, s, BM) + BN - 1) / BN, a.splits, 0,
-                       least).active;
-    p.part0 = (long long)blockIdx.x * a.splits;
-    p.part1 = p.part0 + 1;
-    p.stride = 1;
-  } else {
-    const int l = s.seq - c.base;
-    const int units = __builtin_amdgcn_readlane(c.one, l);
-    p = parts_of(line, h * line.head + c.before +
-                           __builtin_amdgcn_readlane(c.upto, l) -
-                           __builtin_amdgcn_readlane(c.own, l) +
-                           s.row0 / BM * units, units);
-  }
+  p.count = share_of((most_seen(a, s, BM) + MANY_KEYS - 1) / MANY_KEYS,
+                     a.splits, 0, MANY_LEAST).active;
   if (p.count == 1) return;
-  join_rows<K, D, GS>(a, s, h, p, BM, blockIdx.y * ROWS);
+  p.part0 = (long long)blockIdx.x * a.splits;
+  p.part1 = p.part0 + 1;
+  p.stride = 1;
+  join_rows<K, D, GS>(a, s, blockIdx.x % a.Hk, p, BM, blockIdx.y * ROWS);
 }
 
 // ---- launching ------------------------------------------------------------
 
-template <typename K, int D, int GS>
-int launch_join_by(Args& a, int tiles, int BM, int BN, int least,
-                   hipStream_t stream) {
+template <int D, int GS>
+dim3 join_grid(int items, int BM) {
   constexpr int ROWS = 256 / (D / 4) / GS;
-  void* args[] = {&a, &BM, &BN, &least};
-  return (int)hipLaunchKernel(
-      reinterpret_cast<const void*>(&join_kernel<K, D, GS>),
-      dim3(tiles * a.Hk, (BM + ROWS - 1) / ROWS), dim3(256), args, 0, stream);
+  const int n = (BM + ROWS - 1) / ROWS;
+  return dim3(items, BM == 16 && n > 4 ? 4 : n);
+}
+
+// Many parts of few rows: several groups of lanes for a row.
+template <typename K, int D>
+int join_few(Args& a, hipStream_t stream) {
+  void* args[] = {&a};
+  const long long items =
+      (long long)a.Hk * max((long long)a.B, (long long)a.T * a.G / 16);
+  if (a.workers == 1) return 0;
+  return (int)(a.workers / items >= 16
+      ? hipLaunchKernel(
+            reinterpret_cast<const void*>(&join_few_kernel<K, D, 8>),
+            join_grid<D, 8>(a.workers - 1, 16), dim3(256), args, 0, stream)
+      : hipLaunchKernel(
+            reinterpret_cast<const void*>(&join_few_kernel<K, D, 1>),
+            join_grid<D, 1>(a.workers - 1, 16), dim3(256), args, 0, stream));
 }
 
 template <typename K, int D>
-int launch_join(Args& a, int tiles, int BM, int BN, int least,
-                hipStream_t stream) {
-  // many parts of few rows: several groups of lanes for a row
-  const int parts = BN ? a.splits : a.workers / (tiles * a.Hk);
-  return parts >= 16 && tiles * a.Hk * BM <= 4096
-             ? launch_join_by<K, D, 8>(a, tiles, BM, BN, least, stream)
-             : launch_join_by<K, D, 1>(a, tiles, BM, BN, least, stream);
+int join_many(Args& a, int tiles, hipStream_t stream) {
+  void* args[] = {&a};
+  return (int)(a.splits >= 16 && tiles * a.Hk <= 32
+      ? hipLaunchKernel(
+            reinterpret_cast<const void*>(&join_many_kernel<K, D, 8>),
+            join_grid<D, 8>(tiles * a.Hk, 128), dim3(256), args, 0, stream)
+      : hipLaunchKernel(
+            reinterpret_cast<const void*>(&join_many_kernel<K, D, 1>),
+            join_grid<D, 1>(tiles * a.Hk, 128), dim3(256), args, 0, stream));
 }
 
 // workers: of the few kernel, 0 where the many kernel runs; join: whether a
@@ -1403,7 +1430,7 @@ int run(Args a, const Plan& p, hipStream_t stream) {
     int rc = (int)hipLaunchKernel(
         reinterpret_cast<const void*>(&few_kernel<K, D, Q8>),
         dim3(a.workers), dim3(256), args, 0, stream);
-    return rc || !p.join ? rc : launch_join<K, D>(a, tiles, BM, 0, 0, stream);
+    return rc || !p.join ? rc : join_few<K, D>(a, stream);
   }
   a.splits = p.splits;
   a.stats = a.parts + (long long)tiles * a.Hk * a.splits * BM * D;
@@ -1411,8 +1438,7 @@ int run(Args a, const Plan& p, hipStream_t stream) {
   int rc = (int)hipLaunchKernel(
       reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
       dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
-  return rc || a.splits == 1 ? rc
-                             : launch_join<K, D>(a, tiles, BM, 64, 4, stream);
+  return rc || a.splits == 1 ? rc : join_many<K, D>(a, tiles, stream);
 }
 
 template <typename K, bool Q8>

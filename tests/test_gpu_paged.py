@@ -378,7 +378,7 @@ def test_attention_past_32_bits():
 
 
 @pytest.mark.parametrize("most", [3, 200], ids=["few", "many"])
-@pytest.mark.parametrize("count", [65, 300])
+@pytest.mark.parametrize("count", [65, 300, 2500])
 def test_attention_many_sequences(count, most):
     """More sequences than a wave has lanes, empty ones among them."""
 
