@@ -966,9 +966,15 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   constexpr int NL = ROWS >= 16 ? 1 : 16 / ROWS;  // loads for its 16 rows
   constexpr int TILE = BN * D * 2;      // bytes of a tile in LDS
 
-  // K of two tiles, V of two
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  __shared__ int odd_v;  // whether a V value was not finite where it matters
+  // One object, so that the tiles come first: loads to LDS name their place
+  // in 16 bits.
+  static_assert(4 * TILE <= 65536, "tiles past what a load to LDS can name");
+  __shared__ struct {
+    __attribute__((aligned(1024))) char tiles[4 * TILE];  // K of two, V of two
+    int odd_v;  // whether a V value was not finite where it matters
+  } shared;
+  char* const lds = shared.tiles;
+  int& odd_v = shared.odd_v;
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first

@@ -62,11 +62,27 @@ class PagedKVCache:
     v_scale, uint8 [pages, kv_heads, page_size]. page_size is a power of two
     from 16 to 1024, head_dim 32, 64 or 128."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "_pools")
+    __slots__ = ("_tensors", "_pools")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         self._pools = _ext().pools(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = (k, v, k_scale, v_scale)
+
+    @property
+    def k(self):
+        return self._tensors[0]
+
+    @property
+    def v(self):
+        return self._tensors[1]
+
+    @property
+    def k_scale(self):
+        return self._tensors[2]
+
+    @property
+    def v_scale(self):
+        return self._tensors[3]
 
     @property
     def pages(self) -> int:

@@ -94,6 +94,43 @@ def test_read_the_same_slot_twice_and_none():
     paged.kv_write(cache, k[:0], k[:0], none)
 
 
+def test_read_scales_at_the_ends():
+    """255 stands for no value, 0 for 2^-127; fp16 has no value past 65504,
+    which rows of bf16 may have left in a quantised cache."""
+
+    cache = paged.make_cache(1, 16, 1, 32, quantized=True)
+    slots = torch.arange(3, device="cuda")
+    k = torch.full((3, 1, 32), 448.0, device="cuda", dtype=BF16)
+    paged.kv_write(cache, k * 1024, k, slots)
+    assert (cache.k_scale[0, 0, :3] == 137).all()
+    cache.k_scale[0, 0, 1], cache.k_scale[0, 0, 2] = 255, 0
+    got = paged.kv_read(cache, slots)[0].float()
+    assert (got[0] == 448 * 1024).all() and torch.isnan(got[1]).all()
+    assert (got[2] == 448 * 2.0 ** -127).all()
+    half = paged.kv_read(cache, slots, FP16)[0]
+    assert torch.isinf(half[0]).all() and (half[2] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 40], ids=["few", "many"])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@WIDE
+def test_attention_scale_without_a_value(which, n, dtype):
+    """A key or value whose scale byte is 255 makes the rows that see it
+    NaN, and no other."""
+
+    b = Batch([(n, 70), (n, 50)], 4, 2, 64, 16, dtype, True, seed=20)
+    at = int(b.table[0, 69 // 16])
+    getattr(b.cache, which)[at, 1, 69 % 16] = 255
+    got = b.run()
+    assert torch.isnan(got[n - 1, 2:].float()).all()
+    want, tol, mine = Batch([(n, 70), (n, 50)], 4, 2, 64, 16, dtype, True,
+                            seed=20).want()
+    rest = torch.ones_like(want, dtype=torch.bool)
+    rest[n - 1, 2:] = False
+    off = (got.cpu().double() - want).abs() - tol
+    assert off[rest].max() <= 0
+
+
 @pytest.mark.parametrize("layout", ["heads first", "odd start", "odd row"])
 def test_write_any_layout(layout):
     """Strides and addresses that 16-byte loads do not fit."""

@@ -58,6 +58,8 @@ def test_quantized_cache_starts_at_zero():
     assert c.quantized and c.k.float().abs().sum() == 0
     assert (c.k_scale == 127).all()
     assert (c.pages, c.kv_heads, c.page_size, c.head_dim) == (5, 2, 16, 64)
+    with pytest.raises(AttributeError):
+        c.k = c.v  # the operators hold the tensors that it was made with
 
 
 def test_write_refusals():
