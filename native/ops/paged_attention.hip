@@ -153,6 +153,15 @@ __device__ inline float base_of(float m) {
   return m == minus_inf() ? 0.0f : m;
 }
 
+// The maximum that is subtracted is not looked for at every step: p and its
+// sum over a lane's keys are worked out with the one there is, and only where
+// a sum comes out at 2^8 or more (or not as a number: at first the maximum is
+// -inf) is it found and p worked out again. p is then at most 2^8, with the
+// same relative rounding; a maximum that is too high by nothing but age does
+// not occur, since it is some score's. Of 88 vector instructions for 32 keys
+// this saves 20, and the wait for them before the first exponential.
+constexpr float MOST = 256.0f;
+
 __device__ inline f4 mfma16(Bf16::V8 a, Bf16::V8 b, f4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -621,7 +630,7 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   };
 
   f4 o[NT];
-  float m = minus_inf(), sum = 0.0f;
+  float m = seen ? minus_inf() : 0.0f, sum = 0.0f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
 
@@ -734,26 +743,30 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
         if (key >= seen) sc[j >> 2][j & 3] = minus_inf();
       }
     }
-    float top = sc[0][0];
+    auto weigh = [&](float base) {
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
-    top = lane_xor32_max(lane_xor16_max(top)) * scale;
-    // as in the other kernel, the maximum moves by steps of 2^8 or more
-    if (__ballot(top > m + 8.0f)) {
-      const float next = fmaxf(m, top);
-      const float keep = exp2_of(m - base_of(next));
-      m = next;
+      for (int j = 0; j < 8; ++j)
+        p.h[j] = (T)exp2_of(__builtin_fmaf(sc[j >> 2][j & 3], scale, -base));
+      float part = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part = add_pair(p, j, part);
+      return part;
+    };
+    float part = weigh(m);
+    if (__ballot(!(part < MOST))) {
+      float top = sc[0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
+      const float higher =
+          fmaxf(m, lane_xor32_max(lane_xor16_max(top)) * scale);
+      const float keep = exp2_of(m - base_of(higher));
+      m = higher;
       sum *= keep;
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[t] *= keep;
+      part = weigh(base_of(m));
     }
-    const float base = base_of(m);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      p.h[j] = (T)exp2_of(
-          __builtin_fmaf(sc[j >> 2][j & 3], scale, -base));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum = add_pair(p, j, sum);
+    sum += part;
 
     if (look && __ballot(odd_v)) {
       // what is not finite goes to the rows that see it, then gives way
@@ -1155,7 +1168,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   };
 
   f16v o[NT];
-  float m = minus_inf(), sum = 0.0f;
+  float m = seen ? minus_inf() : 0.0f, sum = 0.0f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -1199,14 +1212,24 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
         if (key >= seen) sc[j] = minus_inf();
       }
     }
-    float top = sc[0];
+    scores(next_kd, next);
+    Oct<K> p[2];
+    auto weigh = [&](float base) {
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
-    top = lane_xor32_max(top) * scale;
-    // The sums stay under an old maximum until a score is 2^8 above it:
-    // p is then at most 2^8, with the same relative rounding.
-    if (__ballot(top > m + 8.0f)) {
-      const float higher = fmaxf(m, top);
+      for (int j = 0; j < 16; ++j)
+        p[j >> 3].h[j & 7] =
+            (T)exp2_of(__builtin_fmaf(sc[j], scale, -base));
+      float part = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part = add_pair(p[j >> 2], j & 3, part);
+      return part;
+    };
+    float part = weigh(m);
+    if (__ballot(!(part < MOST))) {
+      float top = sc[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
+      const float higher = fmaxf(m, lane_xor32_max(top) * scale);
       const float keep = exp2_of(m - base_of(higher));
       m = higher;
       sum *= keep;
@@ -1214,19 +1237,13 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[t][j] *= keep;
+      part = weigh(base_of(m));
     }
-    const float base = base_of(m);
-    // while this wave feeds the matrix pipe, the unit's other wave waits
-    // with its own products, and takes the vector pipe
+    sum += part;
+    // While this wave feeds the matrix pipe with nothing else to do, the
+    // unit's other wave waits with its own products, and takes the vector
+    // pipe (8192 tokens: 515 us against 530).
     __builtin_amdgcn_s_setprio(1);
-    scores(next_kd, next);
-    Oct<K> p[2];
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      p[j >> 3].h[j & 7] =
-          (T)exp2_of(__builtin_fmaf(sc[j], scale, -base));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = add_pair(p[j >> 2], j & 3, sum);
     // a lane's 8 keys of a step of 16: 4 hi + 0..3, then 8 + 4 hi + 0..3
 #pragma unroll
     for (int half = 0; half < 2; ++half)
