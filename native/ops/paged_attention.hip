@@ -16,24 +16,34 @@
 // leaves in a lane's registers is, with the keys of a step permuted in V
 // likewise, what P^T takes: p never leaves the registers.
 //
-//   few:  tiles of 16 or 32 rows, 4 waves that each take every fourth tile
-//         of 32 keys by themselves and are joined at the end. K goes from
-//         memory to registers, V through the wave's own LDS and comes back
-//         by transposing reads. Bound by HBM.
+//   few:  tiles of 16 rows, 4 or 8 waves that each take every fourth or
+//         eighth tile of 32 keys by themselves and are joined at the end. K
+//         goes from memory to registers, V through the wave's own LDS and
+//         comes back by transposing reads. An item (a tile of rows and a kv
+//         head) is a workgroup's, or all items are shared out evenly. Bound by
+//         HBM where there is enough to read: 64 sequences of 700 to 8191 keys,
+//         64 / 8 heads, D = 128, 8 bits: 594 MB in 116 us, 5.1 TB/s with the
+//         launches (a large copy reads 6.3); one of 131071 at 16 bits: 537 MB
+//         in 99 us, 5.4 TB/s. Below that by a launch and one way to memory:
+//         8 sequences of 560 keys take 10.3 us, of 128 keys 6.4.
 //   many: tiles of 128 rows, 4 waves of 32 rows over shared tiles of 64
-//         keys in LDS, two of them in turn. Bound by the matrix and vector
-//         pipes.
+//         keys in LDS, two of them in turn. Bound by what the matrix and the
+//         vector pipe issue together: a prompt of 8192 tokens, 32 / 8 heads,
+//         D = 128: 550 GFLOP in 515 to 535 us, 1030 to 1070 TFLOP/s; the
+//         matrix pipe is busy for 54 % and the vector pipe for 43 % of the
+//         time, and a large library product reaches 1180.
 //
-// Both split the keys over gridDim.y where tiles are few; `join` adds the
-// parts. How many splits work is settled on the device, by the sequence's
-// own length.
+// Where that leaves units idle the keys are split: the few kernel's shares
+// end anywhere in an item, the many kernel's over gridDim.y, and a second
+// kernel joins the parts. How many splits work is settled on the device, by
+// the sequence's own length.
 //
 // Keys that a row does not see have p = 0 by selection; V rows past the end
-// enter as 0; where rows of a tile see different keys and V holds NaN or
-// infinities, the tile takes a path that keeps those from rows that do not
-// see them. A page number outside of the pool makes the scores of its keys
-// NaN; a length that the table cannot hold makes its rows NaN. Nothing
-// outside of the tensors is read.
+// enter as 0. Where rows of a tile see different keys, a V value that is NaN
+// or infinite enters the product as 0 and is added by itself to the rows that
+// see it. A page number outside of the pool makes the scores of its keys NaN;
+// a length that the table cannot hold makes its rows NaN. Nothing outside of
+// the tensors is read.
 
 #include "paged_common.h"
 
@@ -54,16 +64,18 @@ struct Args {
   const int* kv_lens;
   const int* table;
   void* out;
-  float* parts;         // [tile * Hk + h][split][row][D]: sums over p v
-  float* stats;         // [tile * Hk + h][split][row][2]: maximum, sum of p
+  // [part][row][D]: sums over p v; [part][row][2]: maximum, sum of p. Parts:
+  // 2 of each worker, or [tile * Hk + h][split]
+  float* parts;
+  float* stats;
   long long q_row, q_head, table_row;
   int cols;  // of the table
   int T, B, Hq, Hk, G, pages, page_log2;
   uint32_t inv_group;  // 2^32 / G, rounded up
   float scale;  // times log2(e): exponentials are of base 2
   int causal, splits;
-  int workers;  // of the few kernel
-  int unit_log2;
+  int workers;    // of the few kernel, where they share the work
+  int unit_log2;  // of their line: 32 << unit_log2 keys
 };
 
 // ---- what is where ----------------------------------------------------
@@ -99,9 +111,9 @@ __device__ inline int most_seen(const Args& a, const Span& s, int rows) {
   return seen_by(a, s, min(rows, s.rows - s.row0) - 1);
 }
 
-// tiles of keys: what this split takes of `all`, and how many splits work
+// tiles of keys: what a workgroup takes of `all`, and how many splits work
 struct Share {
-  int first, last, active;
+  int first, last, active = 1;
 };
 
 // keys of a tile of the many kernel, and the fewest tiles of a split
@@ -156,10 +168,12 @@ __device__ inline float base_of(float m) {
 // The maximum that is subtracted is not looked for at every step: p and its
 // sum over a lane's keys are worked out with the one there is, and only where
 // a sum comes out at 2^8 or more (or not as a number: at first the maximum is
-// -inf) is it found and p worked out again. p is then at most 2^8, with the
-// same relative rounding; a maximum that is too high by nothing but age does
-// not occur, since it is some score's. Of 88 vector instructions for 32 keys
-// this saves 20, and the wait for them before the first exponential.
+// -inf) is it found and p worked out again. So p is at most 2^8 instead of 1:
+// fp16 and 32 bits hold that and the sums with room to spare, and its rounding
+// is relative as before; the maximum itself is always some score's, never too
+// high. Of 88 vector instructions for 32 keys this saves 20, and the wait for
+// them before the first exponential (2 sequences of 2048 new tokens over 6000
+// keys, 32 / 8 heads, D = 128: 400.7 us before, 392 with it).
 constexpr float MOST = 256.0f;
 
 __device__ inline f4 mfma16(Bf16::V8 a, Bf16::V8 b, f4 c) {
@@ -274,9 +288,9 @@ __device__ inline void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// ---- the few rows' work, in equal shares -----------------------------------
+// ---- the few rows' work ----------------------------------------------------
 
-// The work is one line: for each kv head, each sequence, each of its tiles of
+// Shared out, the work is one line: for each kv head, each sequence, each of its tiles of
 // rows, an item of OWN + (its keys / unit keys) units. Worker w takes the
 // units from edge(w) to edge(w + 1): w * per, moved to an item's start or end
 // where that is less than near(item) away. So workers end together however
@@ -285,10 +299,12 @@ __device__ inline void wave_fence() {
 // place 1), and one that it goes on with (place 0). A unit is 32 keys, or
 // more where the line would pass 2^30 units.
 //
-// WHOLE: a workgroup takes 128 keys in 1.1 us, and the kernel that joins two
-// parts takes 4 us; 8 sequences of 560 keys and 8 heads: in two parts 14.8 us,
-// whole 11.6 us.
-constexpr int OWN = 4, NEAR = 4, LEAST = 8, WHOLE = 32;
+// WHOLE: a workgroup of 4 waves takes 128 keys in 1.1 us, and the kernel that
+// joins two parts takes 4.5 us: a part of less than 512 keys does not pay.
+// LEAST: a share holds one of the shortest items at least (8 sequences of 200
+// keys in tables for 8192 take 11.3 us; with 8, by which two came to one
+// workgroup while others had none, 13.3).
+constexpr int OWN = 4, NEAR = 4, LEAST = 5, WHOLE = 32;
 
 __device__ inline int near(int units) {
   return units < WHOLE ? units / 2 + 1 : NEAR;
@@ -311,6 +327,10 @@ struct Line {
   int head, per;  // units of a head's line, of a worker
 };
 
+__device__ inline int length_of(const Args& a, int len) {
+  return len > ((long long)a.cols << a.page_log2) ? -1 : max(len, -1);
+}
+
 __device__ inline Chunk chunk_of(const Args& a, int base, int before,
                                  int BM) {
   const int lane = threadIdx.x & 63, i = base + lane;
@@ -318,8 +338,7 @@ __device__ inline Chunk chunk_of(const Args& a, int base, int before,
   if (i < a.B) {
     c.q0 = min(max(a.q_starts[i], 0), a.T);
     c.n = min(max(a.q_starts[i + 1], 0), a.T) - c.q0;
-    c.len = a.kv_lens[i];
-    if (c.len < 0 || c.len > ((long long)a.cols << a.page_log2)) c.len = -1;
+    c.len = length_of(a, a.kv_lens[i]);
     if (c.n > 0) {
       // at most 2^30 keys: the sum stays below 2^31
       const int log2 = 5 + a.unit_log2;
@@ -341,8 +360,14 @@ __device__ inline Line line_of(const Args& a, Chunk& c, int BM) {
   c = chunk_of(a, 0, 0, BM);
   Line l;
   l.head = __builtin_amdgcn_readlane(c.upto, 63);
-  for (int base = 64; base < a.B; base += 64)
-    l.head += __builtin_amdgcn_readlane(chunk_of(a, base, 0, BM).upto, 63);
+  bool falls = c.n < 0;
+  for (int base = 64; base < a.B; base += 64) {
+    const Chunk x = chunk_of(a, base, 0, BM);
+    l.head += __builtin_amdgcn_readlane(x.upto, 63);
+    falls |= x.n < 0;
+  }
+  // starts that fall could make the line longer than the host knows: no work
+  if (__ballot(falls)) l.head = 0;
   l.per = max((int)((uint32_t)(l.head * a.Hk + a.workers - 1) /
                     (uint32_t)a.workers), LEAST);
   return l;
@@ -410,27 +435,42 @@ __device__ inline Span span_of(const Args& a, const Chunk& c, int seq,
 // Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
 // leaves each at least its own number, needs no sum over the sequences
 // before it, and the last such start at or below `tile` is its sequence.
-__device__ inline Span find(const Args& a, int tile, int BM) {
+// Without their first tiles (FIRST = 0), and without the i, it is as much.
+template <int BM, int FIRST>
+__device__ inline Span find(const Args& a, int tile) {
   // the last 64 sequences whose first one starts at or below the tile
   int base = 0;
   for (int above = (a.B + 63) / 64; above - base > 1;) {
     const int mid = (base + above) / 2;
     const int q0 = min(max(uniform_load(a.q_starts + mid * 64), 0), a.T);
-    if (q0 * a.G / BM + mid * 64 <= tile)
+    if (q0 * a.G / BM + FIRST * mid * 64 <= tile)
       base = mid;
     else
       above = mid;
   }
   const Chunk c = chunk_of(a, base * 64, 0, BM);
   const int lane = threadIdx.x & 63;
-  const int first = c.q0 * a.G / BM + c.base + lane;
+  const int first = c.q0 * a.G / BM + FIRST * (c.base + lane);
   const unsigned long long at =
       __ballot(c.base + lane < a.B && first <= tile);
   if (at == 0) return Span();
   const int last = 63 - __clzll(at);
-  const Span s =
-      span_of(a, c, c.base + last,
-              (tile - __builtin_amdgcn_readlane(first, last)) * BM);
+  const Span s = span_of(
+      a, c, c.base + last,
+      (tile - __builtin_amdgcn_readlane(first, last) + 1 - FIRST) * BM);
+  return s.row0 < s.rows ? s : Span();
+}
+
+// All first tiles, then the others: where no sequence has others, the tiles
+// at the end are those without work, and every unit gets as many with.
+template <int BM>
+__device__ inline Span find_first(const Args& a, int tile) {
+  if (tile >= a.B) return find<BM, 0>(a, tile - a.B);
+  Chunk c{tile, 0, 0, 0, 0, 0, 0, 0};
+  c.q0 = min(max(uniform_load(a.q_starts + tile), 0), a.T);
+  c.n = min(max(uniform_load(a.q_starts + tile + 1), 0), a.T) - c.q0;
+  c.len = length_of(a, uniform_load(a.kv_lens + tile));
+  const Span s = span_of(a, c, tile, 0);
   return s.row0 < s.rows ? s : Span();
 }
 
@@ -519,12 +559,12 @@ __device__ inline int few_piece(int row, int c) {
   return c ^ (((row >> 2) & 1) << 1);
 }
 
-template <typename K, int D, bool Q8>
+template <typename K, int D, bool Q8, int WAVES>
 __device__ inline void
-few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
+few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int h,
          const Share& mine, bool whole, long long part) {
   typedef typename K::T T;
-  constexpr int BM = 16, BN = 32, WAVES = 4;
+  constexpr int BM = 16, BN = 32;
   constexpr int NF = D / 32;              // steps of the product over D
   constexpr int NT = D / 16;              // tiles of 16 values of O^T
   constexpr int EB = Q8 ? 1 : 2;          // bytes of a cached value
@@ -828,7 +868,8 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
   for (int t = 0; t < NT; ++t)
     *reinterpret_cast<f4*>(&all[wave][col][t * 16 + grp * 4]) = o[t];
   __syncthreads();
-  const int row = threadIdx.x >> 4;
+  constexpr int LANES = WAVES * 4;  // for a row
+  const int row = threadIdx.x / LANES;
   if (s.row0 + row >= s.rows) return;
   float top = minus_inf();
 #pragma unroll
@@ -840,15 +881,15 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
     keep[w] = exp2_of(stat[0][w][row] - base);
     total += stat[1][w][row] * keep[w];
   }
-  // pairs of values, 16 lanes a row: stores of one run of memory
-  const int d0 = (threadIdx.x & 15) * 2;
+  // pairs of values: stores of one run of memory
+  const int d0 = threadIdx.x % LANES * 2;
   const Row r = row_at(a, s, row);
   const bool none = seen_by(a, s, row) == 0;
   const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
   T* dst = (T*)a.out + ((long long)(s.q0 + r.t) * a.Hq + h * a.G + r.g) * D;
   const long long at = part * BM + row;
 #pragma unroll
-  for (int d = d0; d < D; d += 32) {
+  for (int d = d0; d < D; d += 2 * LANES) {
     float x = 0.0f, y = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
@@ -868,15 +909,26 @@ few_part(const Args& a, char* lds, float (*stat)[4][16], const Span& s, int h,
     *reinterpret_cast<f2*>(a.stats + at * 2) = f2{top, total};
 }
 
-template <typename K, int D, bool Q8>
-__global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
-  constexpr int BM = 16, BN = 32, WAVES = 4;
+template <typename K, int D, bool Q8, int WAVES, bool SHARED>
+__global__ void __launch_bounds__(WAVES * 64, 2) few_kernel(Args a) {
+  constexpr int BM = 16, BN = 32;
   constexpr int JOIN = WAVES * 16 * (D + 4) * 4, TILES = WAVES * BN * D * 2;
   // V tiles while the keys pass, then the waves' sums
   __shared__ __attribute__((aligned(16))) char
       lds[JOIN > TILES ? JOIN : TILES];
   __shared__ float stat[2][WAVES][16];
 
+  if constexpr (!SHARED) {
+    // an item a workgroup
+    const Span s = find_first<BM>(a, blockIdx.x / a.Hk);
+    if (s.seq < 0) return;
+    Share mine;
+    mine.first = 0;
+    mine.last = (most_seen(a, s, BM) + BN - 1) / BN;
+    few_part<K, D, Q8, WAVES>(a, lds, stat, s, blockIdx.x % a.Hk, mine, true,
+                              0);
+    return;
+  }
   Chunk c;
   const Line line = line_of(a, c, BM);
   if (line.head == 0) return;
@@ -923,7 +975,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(Args a) {
     Share mine;
     mine.first = min(max(from - OWN, 0) << a.unit_log2, all);
     mine.last = min(max(to - OWN, 0) << a.unit_log2, all);
-    few_part<K, D, Q8>(a, lds, stat, s, h, mine,
+    few_part<K, D, Q8, WAVES>(a, lds, stat, s, h, mine,
                        from == 0 && to == it.units,
                        2LL * w + (from == 0 ? 1 : 0));
     if (to < it.units) return;
@@ -991,7 +1043,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
 
   const int h = blockIdx.x % a.Hk;
   const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
-  const Span s = find(a, tile, BM);
+  const Span s = find<BM, 1>(a, tile);
   if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -1387,7 +1439,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(Args a) {
 template <typename K, int D, int GS>
 __global__ void __launch_bounds__(256) join_many_kernel(Args a) {
   constexpr int BM = 128, ROWS = 256 / (D / 4) / GS;
-  const Span s = find(a, blockIdx.x / a.Hk, BM);
+  const Span s = find<BM, 1>(a, blockIdx.x / a.Hk);
   if (s.seq < 0) return;
   Parts p;
   p.count = share_of((most_seen(a, s, BM) + MANY_KEYS - 1) / MANY_KEYS,
@@ -1436,11 +1488,20 @@ int join_many(Args& a, int tiles, hipStream_t stream) {
             join_grid<D, 1>(tiles * a.Hk, 128), dim3(256), args, 0, stream));
 }
 
-// workers: of the few kernel, 0 where the many kernel runs; join: whether a
-// sequence may be long enough for it to be split; splits: of the many kernel.
+// workers: 0 where the many kernel runs; of the few kernel otherwise, of 4 or
+// 8 waves each. join: they share all items out, and a second kernel joins what
+// they split; otherwise an item is a workgroup's. splits: of the many kernel.
 struct Plan {
-  int workers, join, splits;
+  int workers, waves, join, splits;
 };
+
+template <typename K, int D, bool Q8, int WAVES, bool SHARED>
+int few(Args& a, int workgroups, hipStream_t stream) {
+  void* args[] = {&a};
+  return (int)hipLaunchKernel(
+      reinterpret_cast<const void*>(&few_kernel<K, D, Q8, WAVES, SHARED>),
+      dim3(workgroups), dim3(WAVES * 64), args, 0, stream);
+}
 
 template <typename K, int D, bool Q8>
 int run(Args a, const Plan& p, hipStream_t stream) {
@@ -1449,10 +1510,13 @@ int run(Args a, const Plan& p, hipStream_t stream) {
   if (p.workers) {
     a.workers = p.workers;
     a.stats = a.parts + 2LL * a.workers * BM * D;
-    void* args[] = {&a};
-    int rc = (int)hipLaunchKernel(
-        reinterpret_cast<const void*>(&few_kernel<K, D, Q8>),
-        dim3(a.workers), dim3(256), args, 0, stream);
+    const int whole = tiles * a.Hk;
+    const int rc =
+        p.join ? p.waves == 8 ? few<K, D, Q8, 8, true>(a, a.workers, stream)
+                              : few<K, D, Q8, 4, true>(a, a.workers, stream)
+        : Q8 && p.waves == 8
+            ? few<K, D, Q8, Q8 ? 8 : 4, false>(a, whole, stream)
+            : few<K, D, Q8, 4, false>(a, whole, stream);
     return rc || !p.join ? rc : join_few<K, D>(a, stream);
   }
   a.splits = p.splits;
@@ -1479,20 +1543,19 @@ int run_d(const Args& a, const Plan& p, int D, hipStream_t stream) {
 extern "C" {
 
 // parts: 32-bit floats, 2 * workers * 16 * (D + 2) of them where the few
-// kernel's items may be split, tiles * Hk * splits * 128 * (D + 2) for the
-// many kernel's splits.
+// kernel's items are shared out (join), tiles * Hk * splits * 128 * (D + 2)
+// for the many kernel's splits.
 int tf_paged_attention(
     const void* q, const void* k, const void* v, const void* k_scale,
     const void* v_scale, const void* q_starts, const void* kv_lens,
     const void* table, void* out, void* parts, long long q_row,
     long long q_head, long long table_row, int cols, int T, int B, int Hq,
     int Hk, int pages, int page_log2, int D, float scale, int causal,
-    int fp16, int workers, int join, int splits,
-    void* stream) {
+    int fp16, int workers, int waves, int join,
+    int splits, void* stream) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || Hq > 32768 || cols < 0 ||
       pages < 1 || page_log2 < 4 || page_log2 > 10 ||
-      workers < 0 || splits < 1 || splits > 65535 ||
-      (workers && !join && (cols << page_log2) > (WHOLE - 1 - OWN) * 32) ||
+      workers < 0 || (waves != 4 && waves != 8) || splits < 1 || splits > 65535 ||
       ((join || splits > 1) && !parts) ||
       ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
       (long long)T * (Hq / Hk) + 128LL * B >= (1LL << 31))
@@ -1510,7 +1573,7 @@ int tf_paged_attention(
                          (32 << a.unit_log2)) + 1) >= (double)(1 << 30) &&
          a.unit_log2 < 25)
     ++a.unit_log2;
-  const Plan p{workers, join, splits};
+  const Plan p{workers, waves, join, splits};
   const bool q8 = k_scale != nullptr;
   hipStream_t st = (hipStream_t)stream;
   return fp16 ? (q8 ? run_d<Fp16, true>(a, p, D, st)

@@ -40,7 +40,7 @@ int tf_paged_attention(
     const void* table, void* out, void* parts, long long q_row,
     long long q_head, long long table_row, int cols, int T, int B, int Hq,
     int Hk, int pages, int page_log2, int D, float scale, int causal,
-    int fp16, int workers, int join, int splits, void* stream);
+    int fp16, int workers, int waves, int join, int splits, void* stream);
 }
 
 namespace {
@@ -290,7 +290,7 @@ std::pair<Tensor, Tensor> kv_read(const Pools& p, const Tensor& slots,
 }
 
 struct Plan {
-  int64_t workers, join, splits;
+  int64_t workers, waves, join, splits;
 };
 
 // Which kernel attends, and how it shares the keys. What a batch holds lies
@@ -298,6 +298,31 @@ struct Plan {
 // rows (new tokens * G) a sequence are work for the kernel for few rows, whose
 // `workers` share it out among themselves; 0 workers: the kernel for many
 // rows, with the keys of each tile of 128 rows in `splits` parts.
+//
+// Few rows, an item (16 rows or less of a sequence and kv head) a workgroup, or
+// all shared out: an item by itself takes `ns` a key, so where items are too
+// few for the 256 units, or differ, sharing saves that for its keys times the
+// part of the units that idles (taken as a third at least, for lengths that
+// differ); it costs 7 us: 4.5 for the joining kernel, the rest for the search
+// and the parts. Measured (us, D = 128, 8 kv heads, whole against shared):
+// 16 bits, 1 sequence of 700 keys 10.3/14.4, of 1300 15.9/12.7; 8 of 1300
+// 17.8/17.6, of 2400 28.0/20.4; 16 of up to 1300 17.8/21.5, of up to 4000
+// 52.3/41.3; 32 of 1300 33.1/36.1, of up to 2400 44.8/47.9; 64 of up to 1300
+// 45.3/53.9; 8 bits, 8 of 1300 14.0/16.6, of 2400 21.3/17.1; 64 of up to 1300
+// 29.7/40.7; 48 of up to 2400 43.5/41.0.
+//
+// Waves: a unit holds 8 of the few kernel, as one workgroup or as two. Whole
+// items come two to a unit while there are that many, and hide each other's
+// latencies (64 sequences of 250 keys at 8 bits: 4 waves 10.9, 8 waves 14.7).
+// With no more items than units, 8 waves are through with an 8-bit one sooner
+// (8 sequences of 700 keys 13.0/10.1); at 16 bits a unit's loads are what it
+// waits for (8 of 560 11.6/11.6, of 256 8.0/8.5). Shared, one workgroup of 8
+// has half the parts to join (512 of 4 waves against 256 of 8: 64 sequences
+// of 700 to 8191 keys at 8 bits 117.7/115.5, one of 131000 at 16 bits
+// 101.1/99.0, 4 of 1000 in a table for 8192 16.2/13.8), but not where the keys
+// do not give every unit two (2 of 4000 15.2/15.8, 8 of 1699 18.3/19.4). More
+// waves, which D of 32 and 64 have room for, gain nothing (24 sequences of 4000
+// keys, D = 64: 512 workers 30.4, 768 31.9).
 //
 // Splits: a workgroup by itself takes 1.3 us for 64 keys, so s parts save
 // 1.3 us * tiles * (1 - 1/s); they cost 4 us for the joining kernel and the
@@ -309,23 +334,28 @@ struct Plan {
 // 2368 keys: 2 parts 56.2, 3 parts 50.8), unless their tiles are mostly empty
 // and memory is what they wait for (22 rows: 5 parts 32.5, 8 parts 37.2).
 Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
-             int64_t keys) {
+             int64_t keys, bool quantized) {
   const int64_t rows = T * G;
   // of keys that are worth a workgroup
   const int64_t pieces = std::max<int64_t>(1, (keys + 255) / 256);
   if (rows <= 16 * B) {
-    // neighbouring workgroups share an XCD of eight
     const int64_t items = Hk * std::max(B, rows / 16);
-    const int64_t workers = std::min<int64_t>(512, items * pieces);
-    return {(workers + 7) / 8 * 8, keys > 864, 1};  // 864: never split
+    const int waves = quantized && items <= 256 ? 8 : 4;
+    const double ns = !quantized ? 2 + 0.054 * D
+                                 : (1.8 + 0.034 * D) * (waves == 8 ? 1 : 1.7);
+    const double idle = std::max(1 - items / 256.0, 1 / 3.0);
+    if (keys * ns * idle <= 7000) return {Hk * (rows / 16 + B), waves, 0, 1};
+    if (items * pieces >= 512) return {256, 8, 1, 1};
+    // neighbouring workgroups share an XCD of eight
+    return {(items * pieces + 7) / 8 * 8, 4, 1, 1};
   }
   const int64_t busy = Hk * std::max(B, rows / 128);
   const int64_t splits =
       std::min(pieces, (rows >= 64 * B ? 768 : 512) / busy);
-  if (splits <= 1) return {0, 0, 1};
+  if (splits <= 1) return {0, 4, 0, 1};
   const double saved = 1.3 * keys / 64 * (1 - 1.0 / splits);
   const double spent = 4 + (double)rows * Hk * splits * D * 8 / 4e6;
-  return {0, 0, saved > spent ? splits : 1};
+  return {0, 4, 0, saved > spent ? splits : 1};
 }
 
 Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
@@ -370,7 +400,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
   if (T == 0 || B == 0) return out;
   const c10::DeviceGuard guard(p.device);
   q = rows_of(q);
-  const Plan plan = plan_of(T, B, G, Hk, D, cols << p.page_log2);
+  const Plan plan = plan_of(T, B, G, Hk, D, cols << p.page_log2, p.quantized);
   Tensor parts;
   if (plan.join || plan.splits > 1) {
     // its own for every call: two captured graphs never share it
@@ -387,7 +417,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
                q.stride(0), q.stride(1), table.stride(0), (int)cols, (int)T,
                (int)B, (int)Hq, (int)Hk, (int)p.pages, p.page_log2, (int)D,
                (float)scale, causal, q.scalar_type() == at::kHalf,
-               (int)plan.workers, (int)plan.join, (int)plan.splits,
+               (int)plan.workers, (int)plan.waves, (int)plan.join, (int)plan.splits,
                stream_of(p)));
   return out;
 }
@@ -520,7 +550,7 @@ PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count(n, 6);
     const Plan p = plan_of(int_of(a[0], "T"), int_of(a[1], "B"),
                            int_of(a[2], "G"), int_of(a[3], "Hk"),
-                           int_of(a[4], "D"), int_of(a[5], "keys"));
+                           int_of(a[4], "D"), int_of(a[5], "keys"), false);
     return Py_BuildValue("LLL", (long long)p.workers, (long long)p.join,
                          (long long)p.splits);
   });

@@ -244,8 +244,9 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
 
     q: [tokens, heads, head_dim], tokens and heads at any stride, heads a
     multiple of the cache's; q_starts: int32 [B + 1], sequence b's tokens
-    are q_starts[b] .. q_starts[b + 1] - 1; kv_lens: int32 [B], its keys in
-    the cache; block_table: int32 [B, columns], key j lies in page
+    are q_starts[b] .. q_starts[b + 1] - 1, and the starts do not fall (if
+    they do, rows of sequences may be left out); kv_lens: int32 [B], its keys
+    in the cache; block_table: int32 [B, columns], key j lies in page
     block_table[b, j // page_size]. causal: the tokens are the sequence's
     last, and token t of n sees kv_lens[b] - n + t + 1 keys; otherwise each
     sees all. scale: head_dim ** -0.5 if not given. Returns (or fills)

@@ -414,6 +414,31 @@ def test_attention_past_32_bits():
     assert torch.equal(a, k) and torch.equal(b, -k)
 
 
+WHOLE = [(1, 700)] * 30 + [(9, 900), (40, 60), (0, 5), (1, 1)]
+SHARED = [(1, 3000), (2, 2500), (1, 0), (8, 1000), (0, 40)]
+
+
+@pytest.mark.parametrize("seqs,Hk,D,workers", [
+    (WHOLE, 2, 64, 108), (WHOLE * 6, 2, 64, 648), (SHARED, 2, 64, 120),
+    (SHARED * 2, 6, 128, 256)],
+    ids=["whole", "whole, many", "shared", "shared, many"])
+@KEPT
+@WIDE
+def test_attention_few_rows_shared_or_whole(seqs, Hk, D, workers, quantized,
+                                            dtype):
+    """Each way of giving workgroups their work, sequences of several tiles
+    and without tokens among them."""
+
+    b = Batch(seqs, 4 * Hk, Hk, D, 32, dtype, quantized, seed=5)
+    plan = paged._ext().plan(len(b.q), len(seqs), 4, Hk, D,
+                             b.table.shape[1] * 32)
+    assert plan == (workers, seqs[0] == SHARED[0], 1)
+    out = torch.full(b.q.shape, 7.0, dtype=dtype, device="cuda")
+    b.run(out=out)
+    check(out, *b.want())
+    assert torch.equal(b.run(), out)
+
+
 @pytest.mark.parametrize("most", [3, 200], ids=["few", "many"])
 @pytest.mark.parametrize("count", [65, 300, 2500])
 def test_attention_many_sequences(count, most):
