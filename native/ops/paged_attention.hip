@@ -65,7 +65,7 @@ struct Args {
   const int* table;
   void* out;
   // [part][row][D]: sums over p v; [part][row][2]: maximum, sum of p. Parts:
-  // 2 of each worker, or [tile * Hk + h][split]
+  // 2 of each worker, or [tile][h][split]
   float* parts;
   float* stats;
   long long q_row, q_head, table_row;
@@ -74,6 +74,7 @@ struct Args {
   uint32_t inv_group;  // 2^32 / G, rounded up
   float scale;  // times log2(e): exponentials are of base 2
   int causal, splits;
+  int sorted;     // the many kernel's tiles
   int workers;    // of the few kernel, where they share the work
   int unit_log2;  // of their line: 32 << unit_log2 keys
 };
@@ -432,40 +433,74 @@ __device__ inline Span span_of(const Args& a, const Chunk& c, int seq,
   return s;
 }
 
-// Sequence i's tiles of BM rows start at floor(starts[i] * G / BM) + i: that
-// leaves each at least its own number, needs no sum over the sequences
-// before it, and the last such start at or below `tile` is its sequence.
-// Without their first tiles (FIRST = 0), and without the i, it is as much.
+// Places for the tiles of BM rows: sequence i's may start at
+// floor(starts[i] * G / BM) + i, which leaves each at least its own number and
+// needs no sum over the sequences before it; without their first tiles
+// (FIRST = 0), and without the i, it is as much. The 64 sequences that have
+// `place` among theirs:
 template <int BM, int FIRST>
-__device__ inline Span find(const Args& a, int tile) {
-  // the last 64 sequences whose first one starts at or below the tile
+__device__ inline Chunk chunk_at(const Args& a, int place) {
   int base = 0;
   for (int above = (a.B + 63) / 64; above - base > 1;) {
     const int mid = (base + above) / 2;
     const int q0 = min(max(uniform_load(a.q_starts + mid * 64), 0), a.T);
-    if (q0 * a.G / BM + FIRST * mid * 64 <= tile)
+    if (q0 * a.G / BM + FIRST * mid * 64 <= place)
       base = mid;
     else
       above = mid;
   }
-  const Chunk c = chunk_of(a, base * 64, 0, BM);
+  return chunk_of(a, base * 64, 0, BM);
+}
+
+// A tile in the many kernel's order. Where the units get more than two
+// workgroups each, the tiles of the longest of 64 sequences come first, from
+// its last one on: what starts late is short (16 sequences of 52 to 400 new
+// tokens on 498 to 4052 keys, 32 / 8 heads, D = 128: as they come 192 us, like
+// this 173). Otherwise all start at once, the last one first, and are spared
+// the search (12 of 3 to 7 tokens on up to 4000 keys: 37.3 us, with it 38.4).
+template <int BM>
+__device__ inline Span find(const Args& a, int place) {
+  if (!a.sorted) place = a.T * a.G / BM + a.B - 1 - place;
+  const Chunk c = chunk_at<BM, 1>(a, place);
   const int lane = threadIdx.x & 63;
-  const int first = c.q0 * a.G / BM + FIRST * (c.base + lane);
+  const int tiles = c.n > 0 ? (c.n * a.G + BM - 1) / BM : 0;
+  int first = c.q0 * a.G / BM + c.base + lane;
+  if (a.sorted) {
+    first = __builtin_amdgcn_readfirstlane(first);
+    for (int i = 0; i < min(a.B - c.base, 64); ++i) {
+      const int len = __builtin_amdgcn_readlane(c.len, i);
+      if (len > c.len || (len == c.len && i < lane))
+        first += __builtin_amdgcn_readlane(tiles, i);
+    }
+  }
   const unsigned long long at =
-      __ballot(c.base + lane < a.B && first <= tile);
+      __ballot(first <= place && place - first < tiles);
   if (at == 0) return Span();
-  const int last = 63 - __clzll(at);
-  const Span s = span_of(
-      a, c, c.base + last,
-      (tile - __builtin_amdgcn_readlane(first, last) + 1 - FIRST) * BM);
-  return s.row0 < s.rows ? s : Span();
+  const int l = __ffsll(at) - 1;
+  const int back = place - __builtin_amdgcn_readlane(first, l);
+  return span_of(
+      a, c, c.base + l,
+      (a.sorted ? __builtin_amdgcn_readlane(tiles, l) - 1 - back : back) * BM);
 }
 
 // All first tiles, then the others: where no sequence has others, the tiles
 // at the end are those without work, and every unit gets as many with.
 template <int BM>
 __device__ inline Span find_first(const Args& a, int tile) {
-  if (tile >= a.B) return find<BM, 0>(a, tile - a.B);
+  if (tile >= a.B) {
+    tile -= a.B;
+    const Chunk c = chunk_at<BM, 0>(a, tile);
+    const int lane = threadIdx.x & 63;
+    const int first = c.q0 * a.G / BM;
+    const unsigned long long at =
+        __ballot(c.base + lane < a.B && first <= tile);
+    if (at == 0) return Span();
+    const int l = 63 - __clzll(at);
+    const Span s =
+        span_of(a, c, c.base + l,
+                (tile - __builtin_amdgcn_readlane(first, l) + 1) * BM);
+    return s.row0 < s.rows ? s : Span();
+  }
   Chunk c{tile, 0, 0, 0, 0, 0, 0, 0};
   c.q0 = min(max(uniform_load(a.q_starts + tile), 0), a.T);
   c.n = min(max(uniform_load(a.q_starts + tile + 1), 0), a.T) - c.q0;
@@ -1020,7 +1055,7 @@ __device__ inline uint32_t lds_address(const void* p) {
 }
 
 template <typename K, int D, bool Q8>
-__global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
+__global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
   typedef typename K::T T;
   constexpr int BM = 128, BN = MANY_KEYS;
   constexpr int NF = D / 16;            // steps of the product over D
@@ -1042,8 +1077,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
   int& odd_v = shared.odd_v;
 
   const int h = blockIdx.x % a.Hk;
-  const int tile = tiles - 1 - blockIdx.x / a.Hk;  // the longest first
-  const Span s = find<BM, 1>(a, tile);
+  const Span s = find<BM>(a, blockIdx.x / a.Hk);
   if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -1397,8 +1431,8 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a, int tiles) {
         __builtin_memcpy(dst + t * 32 + 2 * j + 4 * hi, y, sizeof y);
       }
   } else {
-    const long long at = ((long long)(tile * a.Hk + h) * a.splits +
-                          blockIdx.y) * BM + wave * 32 + col;
+    const long long at = ((long long)blockIdx.x * a.splits + blockIdx.y) * BM +
+                         wave * 32 + col;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -1439,7 +1473,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(Args a) {
 template <typename K, int D, int GS>
 __global__ void __launch_bounds__(256) join_many_kernel(Args a) {
   constexpr int BM = 128, ROWS = 256 / (D / 4) / GS;
-  const Span s = find<BM, 1>(a, blockIdx.x / a.Hk);
+  const Span s = find<BM>(a, blockIdx.x / a.Hk);
   if (s.seq < 0) return;
   Parts p;
   p.count = share_of((most_seen(a, s, BM) + MANY_KEYS - 1) / MANY_KEYS,
@@ -1506,7 +1540,7 @@ int few(Args& a, int workgroups, hipStream_t stream) {
 template <typename K, int D, bool Q8>
 int run(Args a, const Plan& p, hipStream_t stream) {
   const int BM = p.workers ? 16 : 128;
-  int tiles = (int)((long long)a.T * a.G / BM) + a.B;
+  const int tiles = (int)((long long)a.T * a.G / BM) + a.B;
   if (p.workers) {
     a.workers = p.workers;
     a.stats = a.parts + 2LL * a.workers * BM * D;
@@ -1520,8 +1554,9 @@ int run(Args a, const Plan& p, hipStream_t stream) {
     return rc || !p.join ? rc : join_few<K, D>(a, stream);
   }
   a.splits = p.splits;
+  a.sorted = (long long)tiles * a.Hk * a.splits > 768;
   a.stats = a.parts + (long long)tiles * a.Hk * a.splits * BM * D;
-  void* args[] = {&a, &tiles};
+  void* args[] = {&a};
   int rc = (int)hipLaunchKernel(
       reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
       dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
@@ -1566,7 +1601,7 @@ int tf_paged_attention(
          Hq / Hk, pages, page_log2,
          (uint32_t)(((1ULL << 32) + Hq / Hk - 1) / (Hq / Hk)),
          // 0 times a masked score would be NaN; this leaves every p 1 too
-         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 1, 0};
+         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 0, 1, 0};
   // a line of less than 2^30 units, as bounded by what the host knows
   const double items = ((double)T * (Hq / Hk) / 16 + B) * Hk;
   while (items * (OWN + ((double)cols * (1 << page_log2) /
