@@ -1469,7 +1469,7 @@ __global__ void __launch_bounds__(256) join_few_kernel(Args a) {
   }
 }
 
-// One workgroup for ROWS rows of a tile of the many kernel.
+// Some workgroups for the rows of a tile of the many kernel.
 template <typename K, int D, int GS>
 __global__ void __launch_bounds__(256) join_many_kernel(Args a) {
   constexpr int BM = 128, ROWS = 256 / (D / 4) / GS;
@@ -1482,7 +1482,11 @@ __global__ void __launch_bounds__(256) join_many_kernel(Args a) {
   p.part0 = (long long)blockIdx.x * a.splits;
   p.part1 = p.part0 + 1;
   p.stride = 1;
-  join_rows<K, D, GS>(a, s, blockIdx.x % a.Hk, p, BM, blockIdx.y * ROWS);
+  for (int row = blockIdx.y * ROWS; row < BM && s.row0 + row < s.rows;
+       row += gridDim.y * ROWS) {
+    join_rows<K, D, GS>(a, s, blockIdx.x % a.Hk, p, BM, row);
+    __syncthreads();
+  }
 }
 
 // ---- launching ------------------------------------------------------------
@@ -1491,7 +1495,11 @@ template <int D, int GS>
 dim3 join_grid(int items, int BM) {
   constexpr int ROWS = 256 / (D / 4) / GS;
   const int n = (BM + ROWS - 1) / ROWS;
-  return dim3(items, BM == 16 && n > 4 ? 4 : n);
+  // 4 for an item's rows where there are items for all units, so that the
+  // search for the item counts less (9 prompts and steps, 12 heads, D = 64:
+  // 48.2 us with one for each 16 rows, 47.1 so); otherwise one for each ROWS
+  // (4 sequences of 62 tokens, 15 / 3 heads, D = 128: 33.9 with 4, 27.1)
+  return dim3(items, n > 4 && (BM == 16 || items >= 256) ? 4 : n);
 }
 
 // Many parts of few rows: several groups of lanes for a row.
