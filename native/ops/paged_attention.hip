@@ -34,7 +34,7 @@
 //         time, and a large library product reaches 1180.
 //
 // Where that leaves units idle the keys are split: the few kernel's shares
-// end anywhere in an item, the many kernel's over gridDim.y, and a second
+// end anywhere in an item, the many kernel's in equal parts, and a second
 // kernel joins the parts. How many splits work is settled on the device, by
 // the sequence's own length.
 //
@@ -1076,17 +1076,29 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
   char* const lds = shared.tiles;
   int& odd_v = shared.odd_v;
 
+  // Sorted, a tile's splits come one after the other: the longest tiles' before
+  // the next, and the places without a tile at the end. Otherwise all first
+  // splits, then the second ones. (15 sequences of 13 new tokens, 64 / 8 heads,
+  // D = 64: sorted with the splits outermost 34.6 us, so 30.4; 183 tokens of
+  // one sequence, not sorted: 15.0, with the splits innermost 16.5.)
   const int h = blockIdx.x % a.Hk;
-  const Span s = find<BM>(a, blockIdx.x / a.Hk);
+  int place = blockIdx.x / a.Hk, split = 0;
+  if (a.splits > 1) {
+    const int per = a.sorted ? a.splits : a.T * a.G / BM + a.B;
+    const int major = place / per, minor = place % per;
+    split = a.sorted ? minor : major;
+    place = a.sorted ? major : minor;
+  }
+  const Span s = find<BM>(a, place);
   if (s.seq < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int col = lane & 31, hi = lane >> 5;
 
   const int seen_min = seen_by(a, s, 0), seen_max = most_seen(a, s, BM);
-  const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, blockIdx.y,
+  const Share mine = share_of((seen_max + BN - 1) / BN, a.splits, split,
                               MANY_LEAST);
-  if ((int)blockIdx.y >= mine.active) return;
+  if (split >= mine.active) return;
   if (threadIdx.x == 0) odd_v = 0;
   __syncthreads();
 
@@ -1431,8 +1443,9 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
         __builtin_memcpy(dst + t * 32 + 2 * j + 4 * hi, y, sizeof y);
       }
   } else {
-    const long long at = ((long long)blockIdx.x * a.splits + blockIdx.y) * BM +
-                         wave * 32 + col;
+    const long long at =
+        (((long long)place * a.Hk + h) * a.splits + split) * BM + wave * 32 +
+        col;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -1567,7 +1580,7 @@ int run(Args a, const Plan& p, hipStream_t stream) {
   void* args[] = {&a};
   int rc = (int)hipLaunchKernel(
       reinterpret_cast<const void*>(&many_kernel<K, D, Q8>),
-      dim3(tiles * a.Hk, a.splits), dim3(256), args, 0, stream);
+      dim3(tiles * a.Hk * a.splits), dim3(256), args, 0, stream);
   return rc || a.splits == 1 ? rc : join_many<K, D>(a, tiles, stream);
 }
 
@@ -1601,6 +1614,7 @@ int tf_paged_attention(
       workers < 0 || (waves != 4 && waves != 8) || splits < 1 || splits > 65535 ||
       ((join || splits > 1) && !parts) ||
       ((long long)T * (Hq / Hk) / 16 + B) * Hk >= (1LL << 31) ||
+      ((long long)T * (Hq / Hk) / 128 + B) * Hk >= (1LL << 31) / splits ||
       (long long)T * (Hq / Hk) + 128LL * B >= (1LL << 31))
     return (int)hipErrorInvalidValue;
   Args a{q, k, v, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
