@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <sstream>
@@ -324,15 +325,21 @@ struct Plan {
 // waves, which D of 32 and 64 have room for, gain nothing (24 sequences of 4000
 // keys, D = 64: 512 workers 30.4, 768 31.9).
 //
-// Splits: a workgroup by itself takes 1.3 us for 64 keys, so s parts save
-// 1.3 us * tiles * (1 - 1/s); they cost 4 us for the joining kernel and the
-// way of their sums through memory, at 4 TB/s, there and back. Measured (us,
-// unsplit against split): 184 rows on 272 keys 11.0/13.9, 251 tokens of 64
-// heads on 288 keys 14.7/20.2, 40 tokens of 32 heads on 688 keys 20.2/13.7,
-// 65 tokens of 32 heads on 4032 keys 109/32.5. Two workgroups fit a unit;
-// half more than that balance uneven sequences (295 rows a sequence on up to
-// 2368 keys: 2 parts 56.2, 3 parts 50.8), unless their tiles are mostly empty
-// and memory is what they wait for (22 rows: 5 parts 32.5, 8 parts 37.2).
+// Splits of the many kernel: a workgroup by itself takes 1.3 us for 64 keys, so
+// s parts leave 1/s of 1.3 us * tiles of keys; they cost 4 us for the joining
+// kernel, and s times the way of one part of all sums through memory, at 4 TB/s,
+// there and back. That is least for an s of its own, and bounded by the places
+// for workgroups: two a unit, three for D of 64 and 32. Of few sequences their
+// tiles are known, and to fill the places exactly is best (512 tokens over 8000
+// keys, 32 / 8 heads, D = 128: 4 parts 86.5, 3 parts 91.1, 6 parts 103.8; 2
+// sequences of them: 2 parts 153, 3 parts 178). More sequences are uneven, and
+// half more than two a unit balances them (9 of 295 rows on up to 2353 keys: 2
+// parts 50.8, 3 parts 44.2; 32 of 64 rows on up to 8000: 2 parts 142, 3 parts
+// 112), unless their tiles are mostly empty and memory is what they wait for
+// (15 of 22 rows: 5 parts 32.5, 8 parts 37.2). Unsplit against split: 184 rows
+// on 272 keys 11.0/13.9, 251 tokens of 64 heads on 288 keys 14.7/20.2, 40
+// tokens of 32 heads on 688 keys 20.2/13.7, 65 on 4032 keys 109/32.5; as many
+// as fit against the least: 2 of 64 tokens on 4064 keys 39.5/34.5.
 Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
              int64_t keys, bool quantized) {
   const int64_t rows = T * G;
@@ -349,13 +356,17 @@ Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
     // neighbouring workgroups share an XCD of eight
     return {(items * pieces + 7) / 8 * 8, 4, 1, 1};
   }
-  const int64_t busy = Hk * std::max(B, rows / 128);
-  const int64_t splits =
-      std::min(pieces, (rows >= 64 * B ? 768 : 512) / busy);
-  if (splits <= 1) return {0, 4, 0, 1};
-  const double saved = 1.3 * keys / 64 * (1 - 1.0 / splits);
-  const double spent = 4 + (double)rows * Hk * splits * D * 8 / 4e6;
-  return {0, 4, 0, saved > spent ? splits : 1};
+  const int64_t tiles =
+      Hk * std::max(B, B < 4 ? (rows + 127) / 128 : rows / 128);
+  const int64_t slots = B < 4 ? (D == 128 ? 512 : 768)
+                        : rows < 64 * B ? 512 : 768;
+  const double alone = 1.3 * keys / 64;
+  const double part = (double)rows * Hk * D * 8 / 4e6;
+  const int64_t splits = std::min(
+      {pieces, slots / tiles, (int64_t)std::max(1.0, std::sqrt(alone / part))});
+  if (splits <= 1 || alone * (1 - 1.0 / splits) <= 4 + part * splits)
+    return {0, 4, 0, 1};
+  return {0, 4, 0, splits};
 }
 
 Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
