@@ -439,6 +439,21 @@ def test_attention_few_rows_shared_or_whole(seqs, Hk, D, workers, quantized,
     assert torch.equal(b.run(), out)
 
 
+@KEPT
+def test_attention_sorted_tiles_in_parts(quantized):
+    """More workgroups than places: the longest sequences' tiles first, each
+    in parts; sequences of equal length and without tokens among them."""
+
+    seqs = [(80, 1900), (76, 1500), (95, 300), (0, 50), (80, 80)] * 4
+    b = Batch(seqs, 8, 8, 64, 32, BF16, quantized, seed=6)
+    assert paged._ext().plan(len(b.q), len(seqs), 1, 8, 64,
+                             b.table.shape[1] * 32) == (0, 0, 4)
+    out = torch.full(b.q.shape, 7.0, dtype=BF16, device="cuda")
+    b.run(out=out)
+    check(out, *b.want())
+    assert torch.equal(b.run(), out)
+
+
 @pytest.mark.parametrize("most", [3, 200], ids=["few", "many"])
 @pytest.mark.parametrize("count", [65, 300, 2500])
 def test_attention_many_sequences(count, most):
@@ -533,6 +548,54 @@ def test_captured_steps_replay_as_eager():
         torch.cuda.synchronize()
         for a, w in zip(outs, want):
             assert torch.equal(a, w), i
+
+
+@pytest.mark.parametrize("n", [1, 40], ids=["few", "many"])
+def test_captured_joins_keep_their_own_parts(n):
+    """Two captured graphs whose keys are split, replayed in turn with eager
+    calls between, while lengths and rows change on the device."""
+
+    torch.manual_seed(1)
+    Hq, Hk, D, page, B = 16, 4, 128, 32, 2
+    table = torch.randperm(512, device="cuda").view(B, 256).to(torch.int32)
+    starts = torch.arange(B + 1, device="cuda", dtype=torch.int32) * n
+    lens = torch.full((B,), 5000, device="cuda", dtype=torch.int32)
+    caches = []
+    for q8 in (False, True):
+        c = paged.make_cache(512, page, Hk, D, BF16, q8)
+        k, v = torch.randn(2, 512 * page, Hk, D, device="cuda").to(BF16)
+        paged.kv_write(c, k, v, torch.arange(512 * page, device="cuda"))
+        caches.append(c)
+    rows, workers, splits = n * B * Hq // Hk, *paged._ext().plan(
+        n * B, B, Hq // Hk, Hk, D, 256 * page)[::2]
+    assert workers if rows <= 16 * B else splits > 1
+    qs = [torch.randn(n * B, Hq, D, device="cuda").to(BF16) for _ in caches]
+
+    def call(i):
+        return paged.paged_attention(qs[i], caches[i], starts, lens, table)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for a, b in [(8192, 8100), (n, n), (3000, 8000), (8192, 41), (600, 700)]:
+        lens.copy_(torch.tensor([a, b]))
+        for q in qs:
+            q.copy_(torch.randn_like(q))
+        for g in graphs:
+            g.replay()
+        want = [call(0), call(1)]
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for x, w in zip(outs, want):
+            assert torch.equal(x, w), (a, b)
 
 
 @KEPT
