@@ -265,6 +265,24 @@ def test_attention_scale(scale):
     check(b.run(scale=scale), *b.want(scale=scale))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0, 1e-4])
+@pytest.mark.parametrize("seqs", [STEP, [(1, 9000)], [(2, 9000)]],
+                         ids=["step", "shared", "split"])
+@KEPT
+def test_attention_scale_of_steps(seqs, scale, quantized):
+    heads = 16 if seqs == STEP else 8 * seqs[0][0] ** 3
+    b = Batch(seqs, heads, 4, 128, 64, FP16, quantized, seed=16)
+    check(b.run(scale=scale), *b.want(scale=scale))
+
+
+@pytest.mark.parametrize("seqs", [[(1, 700), (1, 90)], [(3, 400), (0, 8)],
+                                  [(1, 3000)] * 2], ids=str)
+@pytest.mark.parametrize("heads,Hk", [(256, 1), (384, 2), (130, 1)])
+def test_attention_more_heads_than_a_tile_has_rows(seqs, heads, Hk):
+    b = Batch(seqs, heads, Hk, 64, 16, BF16, heads == 384, seed=17)
+    check(b.run(), *b.want())
+
+
 @pytest.mark.parametrize("seqs", [STEP, MANY], ids=["step", "many"])
 def test_attention_far_scores(seqs):
     """Scores of some hundreds: one key takes all, the running maximum
@@ -346,6 +364,17 @@ def test_attention_broken_values_in_masked_places(seqs, value, dtype):
     last = int(b.q_starts[1]) - 1
     assert torch.isnan(got[last, 2:].float()).all()
     check(got, want, tol, mine)
+
+
+@pytest.mark.parametrize("seqs", [[(3, 6000), (2, 900)],
+                                  [(60, 4000), (70, 2000)]],
+                         ids=["shared", "split"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attention_broken_values_where_keys_are_split(seqs, value):
+    workers, _, splits = paged._ext().plan(
+        sum(n for n, _ in seqs), 2, 2, 2, 64, max(k for _, k in seqs))
+    assert workers or splits > 1
+    test_attention_broken_values_in_masked_places(seqs, value, BF16)
 
 
 @pytest.mark.parametrize("seqs", [[(1, 60), (2, 50)], [(150, 150), (40, 90)]],
