@@ -1273,36 +1273,48 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
     for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
 
   // a lane's places in a tile: of K the row `col`, of V the 4 keys by 4
-  // values of its transposing reads
+  // values of its transposing reads. They change over to the other tile by a
+  // bit of theirs, once a tile: worked out for every 32 keys they took a tenth
+  // of the vector instructions (2 sequences of 2048 new tokens over 6000 keys,
+  // 32 / 8 heads, D = 128: 400.9 us, so 393).
   uint32_t k_at[NF], v_at[NT];
+  const int first = (mine.first & 1) * TILE;
 #pragma unroll
   for (int f = 0; f < NF; ++f)
-    k_at[f] = col * (D * 2) + k_piece<D>(col, f * 2 + hi) * 16;
+    k_at[f] = first + col * (D * 2) + k_piece<D>(col, f * 2 + hi) * 16;
   {
     const int row = hi * 4 + ((lane & 15) >> 2);
     const int c = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      v_at[t] = row * (D * 2) + v_piece_at<D>(row, t * 4 + c) * 16 +
-                (lane & 1) * 8;
+      v_at[t] = 2 * TILE + first + row * (D * 2) +
+                v_piece_at<D>(row, t * 4 + c) * 16 + (lane & 1) * 8;
   }
 
-  // S^T of 32 keys, whose K rows start at kd
-  auto scores = [&](const char* kd, f16v& sc) {
+  auto other_k = [&] {
+#pragma unroll
+    for (int f = 0; f < NF; ++f) k_at[f] ^= TILE;
+  };
+  auto other_v = [&] {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v_at[t] ^= TILE;
+  };
+
+  // S^T of the 32 keys from row `row` of the tile
+  auto scores = [&](int row, f16v& sc) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[j] = 0.0f;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       Oct<K> x;
-      x.raw = *reinterpret_cast<const u4*>(kd + k_at[f]);
+      x.raw = *reinterpret_cast<const u4*>(lds + k_at[f] + row * (D * 2));
       sc = mfma32(x.v, q[f].v, sc);
     }
   };
   // The 32 keys from key0 join the sums, while the scores of the next 32 are
   // worked out: what one needs of the vector pipe, the other does not. (Those
   // of no keys at the end, from what lies there, are not used.)
-  auto step = [&](int key0, f16v& sc, const char* vd, const char* next_kd,
-                  f16v& next) {
+  auto step = [&](int key0, f16v& sc, int row, int next_row, f16v& next) {
     if (key0 + 32 > wave_min) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -1310,7 +1322,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
         if (key >= seen) sc[j] = minus_inf();
       }
     }
-    scores(next_kd, next);
+    scores(next_row, next);
     Oct<K> p[2];
     auto weigh = [&](float base) {
 #pragma unroll
@@ -1347,7 +1359,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const char* at = vd + v_at[t] + half * 16 * (D * 2);
+        const char* at = lds + v_at[t] + (row + half * 16) * (D * 2);
         const u2 lo = transposed(at), up = transposed(at + 8 * (D * 2));
         Oct<K> x;
         x.raw = u4{lo[0], lo[1], up[0], up[1]};
@@ -1369,7 +1381,7 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
     if (kt + 1 < mine.last) fetch_k(id2, kt + 1);
   }
   __syncthreads();
-  if (kt < mine.last && kt * BN < wave_max) scores(k_tile(kt), s0);
+  if (kt < mine.last && kt * BN < wave_max) scores(0, s0);
   for (; kt < mine.last; ++kt) {
     const bool more = kt + 1 < mine.last, more2 = kt + 2 < mine.last;
     const int key0 = kt * BN;
@@ -1380,7 +1392,8 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
     }
     if (more) fetch_v(id1, kt + 1);
     if (key0 < wave_max)
-      step(key0, s0, v_tile(kt), k_tile(kt) + 32 * (D * 2), s1);
+      step(key0, s0, 0, 32, s1);
+    other_k();
     if constexpr (!Q8) {
       if (more) put_k(id1, kt + 1, true);
     }
@@ -1390,7 +1403,8 @@ __global__ void __launch_bounds__(256, 2) many_kernel(Args a) {
     }
     if (more2) fetch_k(id2, kt + 2);
     if (key0 + 32 < wave_max)
-      step(key0 + 32, s1, v_tile(kt) + 32 * (D * 2), k_tile(kt + 1), s0);
+      step(key0 + 32, s1, 32, 0, s0);
+    other_v();
     if constexpr (!Q8) {
       if (more) put_v(id1, kt + 1, more2);
     }
