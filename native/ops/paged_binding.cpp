@@ -559,9 +559,13 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     count(n, 6);
-    const Plan p = plan_of(int_of(a[0], "T"), int_of(a[1], "B"),
-                           int_of(a[2], "G"), int_of(a[3], "Hk"),
-                           int_of(a[4], "D"), int_of(a[5], "keys"), false);
+    int64_t x[6];
+    for (int i = 0; i < 6; ++i) {
+      x[i] = int_of(a[i], "a size");
+      if (x[i] < (i < 5) || x[i] > (i < 5 ? 1LL << 18 : 1LL << 30))
+        refuse("no plan for a size of ", x[i]);
+    }
+    const Plan p = plan_of(x[0], x[1], x[2], x[3], x[4], x[5], false);
     return Py_BuildValue("LLL", (long long)p.workers, (long long)p.join,
                          (long long)p.splits);
   });

@@ -170,3 +170,16 @@ def test_plan_covers_every_row(T, B, G):
             assert first >= end
             end = first + -(-(starts[i + 1] - starts[i]) * G // BM)
         assert end <= tiles
+
+
+def test_plan_refuses_what_is_no_size():
+    plan = paged._ext().plan
+    assert plan(1, 1, 1, 1, 128, 0)
+    for i in range(6):
+        sizes = [4, 2, 2, 2, 64, 100]
+        for bad in (-1, 2 ** 40) + ((0,) if i < 5 else ()):
+            sizes[i] = bad
+            with pytest.raises(ValueError, match="no plan"):
+                plan(*sizes)
+    with pytest.raises(ValueError, match="whole number"):
+        plan(1, 1, "x", 1, 1, 1)
