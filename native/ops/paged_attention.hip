@@ -25,7 +25,7 @@
 //         64 / 8 heads, D = 128, 8 bits: 594 MB in 116 us, 5.1 TB/s with the
 //         launches (a large copy reads 6.3); one of 131071 at 16 bits: 537 MB
 //         in 99 us, 5.4 TB/s. Below that by a launch and one way to memory:
-//         8 sequences of 560 keys take 10.3 us, of 128 keys 6.4.
+//         8 sequences of 560 keys take 9.2 us, of 128 keys 5.4.
 //   many: tiles of 128 rows, 4 waves of 32 rows over shared tiles of 64
 //         keys in LDS, two of them in turn. Bound by what the matrix and the
 //         vector pipe issue together: a prompt of 8192 tokens, 32 / 8 heads,
@@ -594,21 +594,21 @@ __device__ inline int few_piece(int row, int c) {
   return c ^ (((row >> 2) & 1) << 1);
 }
 
-template <typename K, int D, bool Q8, int WAVES>
+template <typename K, int D, int DV, bool Q8, int WAVES>
 __device__ inline void
 few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int h,
-         const Share& mine, bool whole, long long part) {
+         int dv, const Share& mine, bool whole, long long part) {
   typedef typename K::T T;
   constexpr int BM = 16, BN = 32;
   constexpr int NF = D / 32;              // steps of the product over D
-  constexpr int NT = D / 16;              // tiles of 16 values of O^T
+  constexpr int NT = DV / 16;             // tiles of 16 values of O^T
   constexpr int EB = Q8 ? 1 : 2;          // bytes of a cached value
-  constexpr int LPR = D * EB / 16;        // lanes for one V row
+  constexpr int LPR = DV * EB / 16;       // lanes for one V row
   constexpr int VROWS = 64 / LPR;         // V rows of one load
   constexpr int NV = BN / VROWS;          // loads for a tile of V
   constexpr int KB = NF * 8 * EB >= 16 ? 16 : 8;  // bytes of a K load
   constexpr int NK = NF * 8 * EB / KB;    // K loads of a lane for 16 keys
-  constexpr int JS = D + 4;               // a row of what the waves join
+  constexpr int JS = DV + 4;              // a row of what the waves join
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int lane = threadIdx.x & 63;
@@ -657,7 +657,7 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
   };
   int id[2];  // pages of the tile to come
   const uint32_t k_off = col * (D * EB) + grp * KB;
-  const uint32_t v_off = lane * 16;
+  const uint32_t v_off = lane / LPR * (D * EB) + lane % LPR * 16 + dv * EB;
 
   auto row_of = [&](int id, int key) {
     const bool bad = (unsigned)id >= (unsigned)a.pages;
@@ -698,8 +698,8 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
         const int vrow = lane / LPR;
         const long long row = (vrow < 16 ? row0 : row1) + (vrow & 15);
         if constexpr (Q8) to.vsr[i] = a.v_scale[row];
-        to.vr[i] = *reinterpret_cast<const u4*>(vc + row * (D * EB) +
-                                             (lane % LPR) * 16);
+        to.vr[i] = *reinterpret_cast<const u4*>(
+            vc + row * (D * EB) + lane % LPR * 16 + dv * EB);
       }
     }
   };
@@ -709,14 +709,14 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
 
-  char* mine_v = lds + wave * (BN * D * 2);
+  char* mine_v = lds + wave * (BN * DV * 2);
   uint32_t v_at[NT];  // a lane's 4 keys by 4 values of transposing reads
   {
     const int row = grp * 4 + (col >> 2);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      v_at[t] = row * (D * 2) +
-                few_piece<D>(row, t * 2 + ((col >> 1) & 1)) * 16 +
+      v_at[t] = row * (DV * 2) +
+                few_piece<DV>(row, t * 2 + ((col >> 1) & 1)) * 16 +
                 (col & 1) * 8;
   }
   // 8-bit tiles: two on their way in turn, since widening one takes long
@@ -794,15 +794,15 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
         widen(y, u2{now.vr[i][2], now.vr[i][3]}, scale);
         if (look) odd_v |= strange(x) || strange(y);
         const int c = (lane % LPR) * 2;
-        char* row = mine_v + vrow * (D * 2);
-        *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c) * 16) = x.raw;
-        *reinterpret_cast<u4*>(row + few_piece<D>(vrow, c + 1) * 16) = y.raw;
+        char* row = mine_v + vrow * (DV * 2);
+        *reinterpret_cast<u4*>(row + few_piece<DV>(vrow, c) * 16) = x.raw;
+        *reinterpret_cast<u4*>(row + few_piece<DV>(vrow, c + 1) * 16) = y.raw;
       } else {
         Oct<K> x;
         x.raw = now.vr[i];
         if (look) odd_v |= strange(x);
-        *reinterpret_cast<u4*>(mine_v + vrow * (D * 2) +
-                               few_piece<D>(vrow, lane % LPR) * 16) = x.raw;
+        *reinterpret_cast<u4*>(mine_v + vrow * (DV * 2) +
+                               few_piece<DV>(vrow, lane % LPR) * 16) = x.raw;
       }
     }
     wave_fence();
@@ -847,10 +847,10 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
       // what is not finite goes to the rows that see it, then gives way
 #pragma unroll 1
       for (int key = 0; key < BN; ++key)
-        each_strange<D>(
+        each_strange<DV>(
             [&](int d) {
-              return (float)*(const T*)(mine_v + key * (D * 2) +
-                                        few_piece<D>(key, d >> 3) * 16 +
+              return (float)*(const T*)(mine_v + key * (DV * 2) +
+                                        few_piece<DV>(key, d >> 3) * 16 +
                                         (d & 7) * 2);
             },
             [&](int d, float v) {
@@ -862,7 +862,7 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
             });
       wave_fence();
 #pragma unroll 1
-      for (int i = lane; i < BN * D / 8; i += 64) {
+      for (int i = lane; i < BN * DV / 8; i += 64) {
         Oct<K>* x = reinterpret_cast<Oct<K>*>(mine_v + i * 16);
         x->raw = finite_only<K>(*x);
       }
@@ -874,7 +874,7 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const u2 lo = transposed(mine_v + v_at[t]);
-      const u2 up = transposed(mine_v + v_at[t] + 16 * (D * 2));
+      const u2 up = transposed(mine_v + v_at[t] + 16 * (DV * 2));
       Oct<K> x;
       x.raw = u4{lo[0], lo[1], up[0], up[1]};
       o[t] = mfma16(x.v, p.v, o[t]);
@@ -921,10 +921,11 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
   const Row r = row_at(a, s, row);
   const bool none = seen_by(a, s, row) == 0;
   const float inv = s.broken ? nan_f32() : none ? 0.0f : 1.0f / total;
-  T* dst = (T*)a.out + ((long long)(s.q0 + r.t) * a.Hq + h * a.G + r.g) * D;
+  T* dst =
+      (T*)a.out + ((long long)(s.q0 + r.t) * a.Hq + h * a.G + r.g) * D + dv;
   const long long at = part * BM + row;
 #pragma unroll
-  for (int d = d0; d < D; d += 2 * LANES) {
+  for (int d = d0; d < DV; d += 2 * LANES) {
     float x = 0.0f, y = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
@@ -944,24 +945,26 @@ few_part(const Args& a, char* lds, float (*stat)[WAVES][16], const Span& s, int 
     *reinterpret_cast<f2*>(a.stats + at * 2) = f2{top, total};
 }
 
-template <typename K, int D, bool Q8, int WAVES, bool SHARED>
+template <typename K, int D, int DV, bool Q8, int WAVES, bool SHARED>
 __global__ void __launch_bounds__(WAVES * 64, 2) few_kernel(Args a) {
   constexpr int BM = 16, BN = 32;
-  constexpr int JOIN = WAVES * 16 * (D + 4) * 4, TILES = WAVES * BN * D * 2;
+  constexpr int JOIN = WAVES * 16 * (DV + 4) * 4, TILES = WAVES * BN * DV * 2;
   // V tiles while the keys pass, then the waves' sums
   __shared__ __attribute__((aligned(16))) char
       lds[JOIN > TILES ? JOIN : TILES];
   __shared__ float stat[2][WAVES][16];
 
   if constexpr (!SHARED) {
-    // an item a workgroup
-    const Span s = find_first<BM>(a, blockIdx.x / a.Hk);
+    // an item a workgroup, or D / DV of them, on one XCD, for its values
+    const int item = blockIdx.x / (8 * D / DV) * 8 + blockIdx.x % 8;
+    const Span s = find_first<BM>(a, item / a.Hk);
     if (s.seq < 0) return;
     Share mine;
     mine.first = 0;
     mine.last = (most_seen(a, s, BM) + BN - 1) / BN;
-    few_part<K, D, Q8, WAVES>(a, lds, stat, s, blockIdx.x % a.Hk, mine, true,
-                              0);
+    few_part<K, D, DV, Q8, WAVES>(a, lds, stat, s, item % a.Hk,
+                                  blockIdx.x / 8 % (D / DV) * DV, mine, true,
+                                  0);
     return;
   }
   Chunk c;
@@ -1010,7 +1013,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) few_kernel(Args a) {
     Share mine;
     mine.first = min(max(from - OWN, 0) << a.unit_log2, all);
     mine.last = min(max(to - OWN, 0) << a.unit_log2, all);
-    few_part<K, D, Q8, WAVES>(a, lds, stat, s, h, mine,
+    few_part<K, D, D, Q8, WAVES>(a, lds, stat, s, h, 0, mine,
                        from == 0 && to == it.units,
                        2LL * w + (from == 0 ? 1 : 0));
     if (to < it.units) return;
@@ -1568,12 +1571,31 @@ struct Plan {
   int workers, waves, join, splits;
 };
 
-template <typename K, int D, bool Q8, int WAVES, bool SHARED>
+template <typename K, int D, int DV, bool Q8, int WAVES, bool SHARED>
 int few(Args& a, int workgroups, hipStream_t stream) {
   void* args[] = {&a};
   return (int)hipLaunchKernel(
-      reinterpret_cast<const void*>(&few_kernel<K, D, Q8, WAVES, SHARED>),
+      reinterpret_cast<const void*>(&few_kernel<K, D, DV, Q8, WAVES, SHARED>),
       dim3(workgroups), dim3(WAVES * 64), args, 0, stream);
+}
+
+// Whole items. Where they are half of the units or less, two or four workgroups
+// take an item: each all of K, and its part of V and of the result, which leaves
+// nothing to join (us, 32 / 8 heads, D = 128, one, two, four: 8 sequences of 700
+// keys 11.6, 11.1, 10.6, at 8 bits 10.1, 8.5, 8.5; 16 of 560 at 8 bits 9.5, 8.2;
+// 1 of 128 6.1, 5.6, 5.2).
+template <typename K, int D, bool Q8>
+int whole(Args& a, const Plan& p, int tiles, hipStream_t stream) {
+  const int items = (tiles * a.Hk + 7) / 8 * 8;  // of each 8, one an XCD
+  const int busy = a.Hk * max(a.B, (int)((long long)a.T * a.G / 16));
+  constexpr int W = Q8 ? 8 : 4;
+  if constexpr (D == 128)
+    if (busy <= 64) return few<K, D, 32, Q8, W, false>(a, items * 4, stream);
+  if constexpr (D >= 64)
+    if (busy <= 128)
+      return few<K, D, D / 2, Q8, W, false>(a, items * 2, stream);
+  return Q8 && p.waves == 8 ? few<K, D, D, Q8, W, false>(a, items, stream)
+                            : few<K, D, D, Q8, 4, false>(a, items, stream);
 }
 
 template <typename K, int D, bool Q8>
@@ -1583,13 +1605,10 @@ int run(Args a, const Plan& p, hipStream_t stream) {
   if (p.workers) {
     a.workers = p.workers;
     a.stats = a.parts + 2LL * a.workers * BM * D;
-    const int whole = tiles * a.Hk;
     const int rc =
-        p.join ? p.waves == 8 ? few<K, D, Q8, 8, true>(a, a.workers, stream)
-                              : few<K, D, Q8, 4, true>(a, a.workers, stream)
-        : Q8 && p.waves == 8
-            ? few<K, D, Q8, Q8 ? 8 : 4, false>(a, whole, stream)
-            : few<K, D, Q8, 4, false>(a, whole, stream);
+        !p.join ? whole<K, D, Q8>(a, p, tiles, stream)
+        : p.waves == 8 ? few<K, D, D, Q8, 8, true>(a, a.workers, stream)
+                       : few<K, D, D, Q8, 4, true>(a, a.workers, stream);
     return rc || !p.join ? rc : join_few<K, D>(a, stream);
   }
   a.splits = p.splits;

@@ -306,18 +306,18 @@ struct Plan {
 // part of the units that idles (taken as a third at least, for lengths that
 // differ); it costs 7 us: 4.5 for the joining kernel, the rest for the search
 // and the parts. Measured (us, D = 128, 8 kv heads, whole against shared):
-// 16 bits, 1 sequence of 700 keys 10.3/14.4, of 1300 15.9/12.7; 8 of 1300
-// 17.8/17.6, of 2400 28.0/20.4; 16 of up to 1300 17.8/21.5, of up to 4000
-// 52.3/41.3; 32 of 1300 33.1/36.1, of up to 2400 44.8/47.9; 64 of up to 1300
-// 45.3/53.9; 8 bits, 8 of 1300 14.0/16.6, of 2400 21.3/17.1; 64 of up to 1300
-// 29.7/40.7; 48 of up to 2400 43.5/41.0.
+// 16 bits, 1 sequence of 700 keys 9.3/14.4, of 1300 14.3/12.7; 8 of 1300
+// 16.6/17.4, of 2400 26.7/20.1; 16 of up to 1300 17.2/21.5, of up to 4000
+// 44.2/41.4; 32 of 1300 33.1/36.1, of up to 2400 44.8/47.9; 64 of up to 1300
+// 45.3/53.9; 8 bits, 8 of 1300 12.0/16.3, of 2400 17.2/17.2; 16 of 2400
+// 18.2/22.8; 64 of up to 1300 29.7/40.7; 48 of up to 2400 43.5/41.0.
 //
 // Waves: a unit holds 8 of the few kernel, as one workgroup or as two. Whole
 // items come two to a unit while there are that many, and hide each other's
 // latencies (64 sequences of 250 keys at 8 bits: 4 waves 10.9, 8 waves 14.7).
 // With no more items than units, 8 waves are through with an 8-bit one sooner
-// (8 sequences of 700 keys 13.0/10.1); at 16 bits a unit's loads are what it
-// waits for (8 of 560 11.6/11.6, of 256 8.0/8.5). Shared, one workgroup of 8
+// (8 sequences of 700 keys, a workgroup an item: 13.0/10.1); at 16 bits a unit's
+// loads are what it waits for (8 of 560 11.6/11.6, of 256 8.0/8.5). Shared, one workgroup of 8
 // has half the parts to join (512 of 4 waves against 256 of 8: 64 sequences
 // of 700 to 8191 keys at 8 bits 117.7/115.5, one of 131000 at 16 bits
 // 101.1/99.0, 4 of 1000 in a table for 8192 16.2/13.8), but not where the keys
@@ -348,8 +348,10 @@ Plan plan_of(int64_t T, int64_t B, int64_t G, int64_t Hk, int64_t D,
   if (rows <= 16 * B) {
     const int64_t items = Hk * std::max(B, rows / 16);
     const int waves = quantized && items <= 256 ? 8 : 4;
-    const double ns = !quantized ? 2 + 0.054 * D
-                                 : (1.8 + 0.034 * D) * (waves == 8 ? 1 : 1.7);
+    const double ns = !quantized     ? 2 + 0.054 * D
+                      : items <= 128 ? std::min(1.8 + 0.034 * D, 4.3)
+                      : items <= 256 ? 1.8 + 0.034 * D
+                                     : 3.1 + 0.058 * D;
     const double idle = std::max(1 - items / 256.0, 1 / 3.0);
     if (keys * ns * idle <= 7000) return {Hk * (rows / 16 + B), waves, 0, 1};
     if (items * pieces >= 512) return {256, 8, 1, 1};

@@ -448,9 +448,11 @@ SHARED = [(1, 3000), (2, 2500), (1, 0), (8, 1000), (0, 40)]
 
 
 @pytest.mark.parametrize("seqs,Hk,D,workers", [
-    (WHOLE, 2, 64, 108), (WHOLE * 6, 2, 64, 648), (SHARED, 2, 64, 120),
+    (WHOLE, 2, 64, 108), (WHOLE, 3, 128, 162), (WHOLE, 1, 128, 54),
+    (WHOLE * 6, 2, 64, 648), (WHOLE * 6, 2, 128, 648), (SHARED, 2, 64, 120),
     (SHARED * 2, 6, 128, 256)],
-    ids=["whole", "whole, many", "shared", "shared, many"])
+    ids=["two an item", "two an item, 128", "four an item", "one an item",
+         "one an item, 128", "shared", "shared, many"])
 @KEPT
 @WIDE
 def test_attention_few_rows_shared_or_whole(seqs, Hk, D, workers, quantized,
