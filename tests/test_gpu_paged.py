@@ -444,11 +444,12 @@ def test_attention_past_32_bits():
 
 
 WHOLE = [(1, 700)] * 30 + [(9, 900), (40, 60), (0, 5), (1, 1)]
+SHORT = [(1, 500)] * 30 + [(9, 600), (40, 60), (0, 5), (1, 1)]
 SHARED = [(1, 3000), (2, 2500), (1, 0), (8, 1000), (0, 40)]
 
 
 @pytest.mark.parametrize("seqs,Hk,D,workers", [
-    (WHOLE, 2, 64, 108), (WHOLE, 3, 128, 162), (WHOLE, 1, 128, 54),
+    (WHOLE, 2, 64, 108), (WHOLE, 3, 128, 162), (SHORT, 1, 128, 54),
     (WHOLE * 6, 2, 64, 648), (WHOLE * 6, 2, 128, 648), (SHARED, 2, 64, 120),
     (SHARED * 2, 6, 128, 256)],
     ids=["two an item", "two an item, 128", "four an item", "one an item",
