@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -89,10 +90,35 @@ PyTypeObject* pools_type = nullptr;
 
 bool wide(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 
+// A kernel is given addresses: what lies there has to be the tensor's values.
+// It is not where a Python class or a function transform stands between (fake,
+// distributed and batched tensors), where a sign is still to be applied, or
+// where the storage has been taken away.
+void check_plain(const char* name, const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet between(
+      {DispatchKey::Python, DispatchKey::Functionalize,
+       DispatchKey::FuncTorchGradWrapper, DispatchKey::FuncTorchBatched,
+       DispatchKey::Batched, DispatchKey::ZeroTensor, DispatchKey::Negative,
+       DispatchKey::Conjugate});
+  if (t.layout() != at::kStrided || t.is_nested() ||
+      t.key_set().has_any(between) ||
+      (t.numel() && at::detail::computeStorageNbytes(
+                        t.sizes(), t.strides(), t.itemsize(),
+                        t.storage_offset()) > t.storage().nbytes()))
+    refuse(name, " is a plain tensor: dense, with its values in its memory");
+}
+
+// what is allocated here: under a mode that fakes tensors, so is that
+Tensor fresh(Tensor t) {
+  check_plain("a result", t);
+  return t;
+}
+
 Tensor tensor_of(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(name, " is a tensor");
   Tensor t = THPVariable_Unpack(o);
-  if (t.layout() != at::kStrided) refuse(name, " is a dense tensor");
+  check_plain(name, t);
   return t;
 }
 
@@ -186,7 +212,7 @@ void check_index(const char* name, const Tensor& x, int64_t n) {
 Tensor rows_of(const Tensor& x) {
   bool fits = x.stride(-1) == 1 && aligned(x);
   for (int64_t i = 0; i + 1 < x.dim(); ++i) fits = fits && x.stride(i) % 8 == 0;
-  return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+  return fits ? x : fresh(x.clone(at::MemoryFormat::Contiguous));
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -258,7 +284,8 @@ Tensor rope_kv_write(const Pools& p, Tensor q_in, Tensor k_in, Tensor v_in,
   no_grad({&q_in, &k_in, &v_in});
   on_gpu(p, {&q_in, &k_in, &v_in, &cos, &sin, &pos, &slots});
   const c10::DeviceGuard guard(p.device);
-  Tensor q = at::empty({n, heads, D}, q_in.options().requires_grad(false));
+  Tensor q =
+      fresh(at::empty({n, heads, D}, q_in.options().requires_grad(false)));
   if (n == 0) return q;
   q_in = rows_of(q_in);
   k_in = rows_of(k_in);
@@ -279,8 +306,8 @@ std::pair<Tensor, Tensor> kv_read(const Pools& p, const Tensor& slots,
   if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   const c10::DeviceGuard guard(p.device);
   const auto options = p.k.options().dtype(dtype);
-  Tensor k = at::empty({n, p.kv_heads, p.D}, options);
-  Tensor v = at::empty({n, p.kv_heads, p.D}, options);
+  Tensor k = fresh(at::empty({n, p.kv_heads, p.D}, options));
+  Tensor v = fresh(at::empty({n, p.kv_heads, p.D}, options));
   if (n)
     launched("tf_paged_read",
              tf_paged_read(ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale),
@@ -403,7 +430,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
   no_grad({&q});
   on_gpu(p, {&q, &starts, &lens, &table});
   if (!out.defined())
-    out = at::empty({T, Hq, D}, q.options().requires_grad(false));
+    out = fresh(at::empty({T, Hq, D}, q.options().requires_grad(false)));
   else if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() ||
            !out.is_contiguous() || out.device() != q.device() ||
            !aligned(out))
@@ -420,8 +447,8 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
     const int64_t rows = plan.workers
                              ? 2 * plan.workers * 16
                              : (T * G / 128 + B) * Hk * plan.splits * 128;
-    parts = at::empty({rows * (D + 2)},
-                      q.options().dtype(at::kFloat).requires_grad(false));
+    parts = fresh(at::empty({rows * (D + 2)}, q.options().dtype(at::kFloat)
+                                                  .requires_grad(false)));
   }
   launched("tf_paged_attention",
            tf_paged_attention(

@@ -18,9 +18,10 @@ The operators serve: they have no backward pass and refuse inputs that ask
 for one. They run on the current stream of the tensors' device and never
 wait for the GPU; lengths, slots and tables stay on the device, so that a
 captured graph is replayed while they change. Shapes, types and devices are
-checked on the host (ValueError); what lies on the device is checked by the kernels,
-which read and write nothing outside of the tensors: see each operator for
-what they answer instead.
+checked on the host (ValueError), and that the tensors are plain ones, with
+their values in their memory; what lies on the device is checked by the
+kernels, which read and write nothing outside of the tensors: see each
+operator for what they answer instead.
 """
 from __future__ import annotations
 
