@@ -215,6 +215,19 @@ Tensor rows_of(const Tensor& x) {
   return fits ? x : fresh(x.clone(at::MemoryFormat::Contiguous));
 }
 
+// whether any byte between the first and the last of one lies there of another
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return false;
+  auto at = [](const Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr());
+  };
+  auto bytes = [](const Tensor& t) {
+    return at::detail::computeStorageNbytes(t.sizes(), t.strides(),
+                                            t.itemsize());
+  };
+  return at(a) < at(b) + bytes(b) && at(b) < at(a) + bytes(a);
+}
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 void* stream_of(const Pools& p) {
@@ -428,18 +441,25 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
     refuse(T, " tokens of ", Hq, " heads: too many for a launch");
   if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)D);
   no_grad({&q});
+  if (out.defined()) {
+    if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() ||
+        !out.is_contiguous() || out.device() != q.device() || !aligned(out))
+      refuse("out has q's shape, type and device, without gaps");
+    no_grad({&out});
+    for (const Tensor* x :
+         {&p.k, &p.v, &p.k_scale, &p.v_scale, &starts, &lens, &table})
+      if (overlap(out, *x))
+        refuse("out shares memory with the cache, the starts, the lengths or "
+               "the table");
+  }
   on_gpu(p, {&q, &starts, &lens, &table});
   if (!out.defined())
     out = fresh(at::empty({T, Hq, D}, q.options().requires_grad(false)));
-  else if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() ||
-           !out.is_contiguous() || out.device() != q.device() ||
-           !aligned(out))
-    refuse("out has q's shape, type and device, without gaps");
-  else
-    no_grad({&out});
   if (T == 0 || B == 0) return out;
   const c10::DeviceGuard guard(p.device);
-  q = rows_of(q);
+  // several workgroups may read a row that one of them answers
+  q = overlap(out, q) ? fresh(q.clone(at::MemoryFormat::Contiguous))
+                      : rows_of(q);
   const Plan plan = plan_of(T, B, G, Hk, D, cols << p.page_log2, p.quantized);
   Tensor parts;
   if (plan.join || plan.splits > 1) {

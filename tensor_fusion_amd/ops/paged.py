@@ -251,7 +251,8 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
     block_table[b, j // page_size]. causal: the tokens are the sequence's
     last, and token t of n sees kv_lens[b] - n + t + 1 keys; otherwise each
     sees all. scale: head_dim ** -0.5 if not given. Returns (or fills)
-    out [tokens, heads, head_dim].
+    out [tokens, heads, head_dim], which may be q or share memory with it (q
+    is copied then), but not with the cache or the other tensors.
 
     A row that sees no key is 0. Rows before q_starts[0] and from
     q_starts[B] on are left as they were. A row that sees a key whose page

@@ -28,3 +28,36 @@ def test_results_under_a_mode_that_fakes_tensors():
         with pytest.raises(ValueError, match="plain tensor"):
             paged.kv_read(b.cache, slots)
     check(paged.paged_attention(q, b.cache, starts, lens, table), *b.want())
+
+
+# ---- results over what is read ------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,D,seqs", [
+    (8, 64, [(1, 300), (1, 90), (1, 500)]),
+    (8, 128, [(1, 300), (1, 90), (1, 500)]),
+    (8, 64, [(1, 300)] * 40), (16, 128, [(2, 300)] * 40),
+    (8, 64, [(1, 4000), (2, 3000)]), (8, 128, [(150, 150), (70, 400)]),
+    (8, 64, [(40, 3000), (30, 2900)])],
+    ids=["two an item", "four an item", "two, 40", "one an item", "shared",
+         "many", "many in parts"])
+@KEPT
+def test_out_is_q(heads, D, seqs, quantized):
+    """In place, and moved by some rows to either side: several workgroups
+    read the rows that one of them writes."""
+
+    b = Batch(seqs, heads, 2 if heads == 8 else 4, D, 16, BF16, quantized,
+              seed=D)
+    want = b.run()
+    starts, lens, table = b.q_starts.cuda(), b.kv_lens.cuda(), b.table.cuda()
+    T = len(b.q)
+    flat = torch.empty(3 * T, heads, D, dtype=BF16, device="cuda")
+    for first in (T, T - 1, T + 1, T - 1 - T // 2):
+        flat.fill_(7.0)
+        q, out = flat[T:2 * T], flat[first:first + T]
+        q.copy_(b.q)
+        assert paged.paged_attention(q, b.cache, starts, lens, table,
+                                     out=out) is out
+        assert torch.equal(out, want)
+        assert (flat[:min(first, T)] == 7).all()
+        assert (flat[max(first, T) + T:] == 7).all()

@@ -97,3 +97,37 @@ def test_fake_tensors(device):
         q = torch.zeros(3, 4, 64, dtype=BF16, device=device)
     with pytest.raises(ValueError, match="plain tensor"):
         attend(c, q)
+
+
+# ---- results over what is read ------------------------------------------------
+
+
+@pytest.mark.parametrize("pool", ["k", "v", "k_scale", "v_scale"])
+def test_out_over_the_cache(pool):
+    """From the byte behind it to the byte before it, and not next to it."""
+
+    c = cache(quantized=True)
+    parts = {p: getattr(c, p) for p in ("k", "v", "k_scale", "v_scale")}
+    x, size = parts[pool], 3 * 4 * 64 * 2
+    flat = torch.zeros(2 * size + x.numel(), dtype=torch.uint8)
+    parts[pool] = flat[size:size + x.numel()].view(x.dtype).view(x.shape)
+    c = paged.PagedKVCache(*parts.values())
+    last = size + x.numel()
+    for first, match in ((0, "run on a GPU"), (16, "shares"),
+                         (last - 16, "shares"), (last, "run on a GPU")):
+        out = flat[first:first + size].view(BF16).view(3, 4, 64)
+        with pytest.raises(ValueError, match=match):
+            attend(c, out=out)
+
+
+def test_out_over_the_lengths():
+    flat = torch.zeros(3 * 4 * 64, dtype=BF16)
+    ints = flat.view(I32)
+    out = flat.view(3, 4, 64)
+    a = dict(starts=torch.zeros(3, dtype=I32), lens=torch.zeros(2, dtype=I32),
+             table=torch.zeros(2, 3, dtype=I32))
+    over = dict(starts=ints[8:11], lens=ints[-2:], table=ints[:6].view(2, 3))
+    for name, x in over.items():
+        with pytest.raises(ValueError, match="shares"):
+            paged.paged_attention(rows(heads=4), cache(),
+                                  *{**a, name: x}.values(), out=out)
