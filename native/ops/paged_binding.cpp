@@ -228,6 +228,14 @@ bool overlap(const Tensor& a, const Tensor& b) {
   return at(a) < at(b) + bytes(b) && at(b) < at(a) + bytes(a);
 }
 
+// rows to be written, and not from under them: rows that lie in the cache are
+// copied before
+Tensor source_of(const Pools& p, const Tensor& x) {
+  for (const Tensor* pool : {&p.k, &p.v, &p.k_scale, &p.v_scale})
+    if (overlap(x, *pool)) return fresh(x.clone(at::MemoryFormat::Contiguous));
+  return rows_of(x);
+}
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 void* stream_of(const Pools& p) {
@@ -266,8 +274,8 @@ void kv_write(const Pools& p, Tensor k, Tensor v, const Tensor& slots) {
   if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   if (n == 0) return;
   const c10::DeviceGuard guard(p.device);
-  k = rows_of(k);
-  v = rows_of(v);
+  k = source_of(p, k);
+  v = source_of(p, v);
   write(p, Tensor(), k, v, k.stride(1), v.stride(1), Tensor(), Tensor(),
         Tensor(), slots, Tensor(), (int)n, 0);
 }
@@ -300,9 +308,9 @@ Tensor rope_kv_write(const Pools& p, Tensor q_in, Tensor k_in, Tensor v_in,
   Tensor q =
       fresh(at::empty({n, heads, D}, q_in.options().requires_grad(false)));
   if (n == 0) return q;
-  q_in = rows_of(q_in);
-  k_in = rows_of(k_in);
-  v_in = rows_of(v_in);
+  q_in = source_of(p, q_in);
+  k_in = source_of(p, k_in);
+  v_in = source_of(p, v_in);
   write(p, q_in, k_in, v_in, D, D, cos, sin, pos, slots, q, (int)n,
         (int)heads);
   return q;

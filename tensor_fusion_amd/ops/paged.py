@@ -209,7 +209,7 @@ def kv_write(cache: PagedKVCache, k, v, slots) -> None:
     are held to +-61440, the last e4m3 step that fp16 has. Rows whose slot
     is negative (padding) or past the pool are not written. Slots that are
     written have to differ: of two rows for one slot, parts of either may
-    stay."""
+    stay. Rows may lie in the cache themselves: they are copied first."""
 
     (_EXT or _ext()).kv_write(cache._pools, k, v, slots)
 

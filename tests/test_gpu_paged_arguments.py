@@ -61,3 +61,49 @@ def test_out_is_q(heads, D, seqs, quantized):
         assert torch.equal(out, want)
         assert (flat[:min(first, T)] == 7).all()
         assert (flat[max(first, T) + T:] == 7).all()
+
+
+# ---- rows that lie in the cache themselves --------------------------------------
+
+
+@pytest.mark.parametrize("heads,D", [(2, 64), (8, 128), (1, 32)])
+def test_write_rows_of_the_cache(heads, D):
+    """Tokens moved on by some slots, over each other: every row is written
+    as it was before the call."""
+
+    page, pages = 64, 40
+    cache = paged.make_cache(pages, page, heads, D)
+    n = pages * page
+    k, v = torch.randn(2, n, heads, D, device="cuda").to(BF16)
+    slots = torch.arange(n, device="cuda")
+    for by in (1, 17, -3, 700):
+        paged.kv_write(cache, k, v, slots)
+        to = (slots + by) % n
+        # the first page's rows, in order
+        rows = [x[0].transpose(0, 1) for x in (cache.k, cache.v)]
+        paged.kv_write(cache, *rows, to[:page])
+        got = paged.kv_read(cache, slots)
+        for x, new in zip(got, (k, v)):
+            want = new.clone()
+            want[to[:page]] = new[:page]
+            assert torch.equal(x, want), by
+
+
+def test_rope_rows_of_the_cache():
+    """q and k of a product that lies where the pages are."""
+
+    D, Hk, heads, n = 64, 2, 4, 512
+    angle = torch.rand(n, D // 2, device="cuda")
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.arange(n, device="cuda")
+    x = torch.randn(n, (heads + 2 * Hk) * D, device="cuda").to(BF16)
+    apart, over = (paged.make_cache(n // 16 * 4, 16, Hk, D) for _ in "ab")
+    rows = over.k.view(-1, (heads + 2 * Hk) * D)[:n]
+    rows.copy_(x)
+    slots = torch.randperm(4 * n, device="cuda")[:n]
+    outs = [paged.rope_kv_write(c, *r.split([heads * D, Hk * D, Hk * D], 1),
+                                cos, sin, pos, slots, heads)
+            for c, r in ((apart, x), (over, rows))]
+    assert torch.equal(*outs)
+    for a, b in zip(paged.kv_read(apart, slots), paged.kv_read(over, slots)):
+        assert torch.equal(a, b)
