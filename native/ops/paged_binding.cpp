@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -183,12 +184,16 @@ void on_gpu(const Pools& p, std::initializer_list<const Tensor*> all) {
     refuse("the paged operators run on a GPU: got ", p.device);
 }
 
+// neither a backward pass nor a tangent
 void no_grad(std::initializer_list<const Tensor*> all) {
-  if (!at::GradMode::is_enabled()) return;
+  const bool backward = at::GradMode::is_enabled(),
+             forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : all)
-    if (t->requires_grad())
-      throw NoBackward("the paged operators have no backward pass: call them "
-                       "under torch.no_grad()");
+    if (t->defined() && ((backward && t->requires_grad()) ||
+                         (forward && t->_fw_grad(0).defined())))
+      throw NoBackward("the paged operators have no backward pass and no "
+                       "forward mode: call them under torch.no_grad(), and "
+                       "without tangents");
 }
 
 void check_rows(const Pools& p, std::initializer_list<const Tensor*> all) {
@@ -269,7 +274,7 @@ void kv_write(const Pools& p, Tensor k, Tensor v, const Tensor& slots) {
     refuse("k and v are ", Shape{want}, ": got ", shape(k), " and ", shape(v));
   check_rows(p, {&k, &v});
   check_index("slots", slots, n);
-  no_grad({&k, &v});
+  no_grad({&k, &v, &p.k, &p.v});
   on_gpu(p, {&k, &v, &slots});
   if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   if (n == 0) return;
@@ -302,7 +307,7 @@ Tensor rope_kv_write(const Pools& p, Tensor q_in, Tensor k_in, Tensor v_in,
   check_index("slots", slots, n);
   if (heads + 2 * p.kv_heads > 65535 || n >= (1LL << 31))
     refuse("too many heads (", heads, ") or rows (", n, ")");
-  no_grad({&q_in, &k_in, &v_in});
+  no_grad({&q_in, &k_in, &v_in, &cos, &sin, &p.k, &p.v});
   on_gpu(p, {&q_in, &k_in, &v_in, &cos, &sin, &pos, &slots});
   const c10::DeviceGuard guard(p.device);
   Tensor q =
@@ -323,6 +328,7 @@ std::pair<Tensor, Tensor> kv_read(const Pools& p, const Tensor& slots,
   if (slots.dim() != 1) refuse("slots is int64 [n]: got ", shape(slots));
   const int64_t n = slots.size(0);
   check_index("slots", slots, n);
+  no_grad({&p.k, &p.v});
   on_gpu(p, {&slots});
   if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   const c10::DeviceGuard guard(p.device);
@@ -448,12 +454,11 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
       (T * G / 16 + B) * Hk >= most)
     refuse(T, " tokens of ", Hq, " heads: too many for a launch");
   if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)D);
-  no_grad({&q});
+  no_grad({&q, &out, &p.k, &p.v});
   if (out.defined()) {
     if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() ||
         !out.is_contiguous() || out.device() != q.device() || !aligned(out))
       refuse("out has q's shape, type and device, without gaps");
-    no_grad({&out});
     for (const Tensor* x :
          {&p.k, &p.v, &p.k_scale, &p.v_scale, &starts, &lens, &table})
       if (overlap(out, *x))

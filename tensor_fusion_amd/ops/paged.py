@@ -14,8 +14,8 @@ A pool is bf16, fp16, or e4m3 with one scale a token and head (`quantized`):
 a byte s for 2**(s - 127), the smallest power of two with
 max|x| <= 448 * scale. The value that a code stands for is code * scale.
 
-The operators serve: they have no backward pass and refuse inputs that ask
-for one. They run on the current stream of the tensors' device and never
+The operators serve: they have no backward pass and no forward mode, and
+refuse tensors that ask for either. They run on the current stream of the tensors' device and never
 wait for the GPU; lengths, slots and tables stay on the device, so that a
 captured graph is replayed while they change. Shapes, types and devices are
 checked on the host (ValueError), and that the tensors are plain ones, with

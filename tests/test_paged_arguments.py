@@ -2,6 +2,7 @@
 needed. Each is refused before anything is launched."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tensor_fusion_amd.ops import paged
@@ -131,3 +132,45 @@ def test_out_over_the_lengths():
         with pytest.raises(ValueError, match="shares"):
             paged.paged_attention(rows(heads=4), cache(),
                                   *{**a, name: x}.values(), out=out)
+
+
+# ---- gradients in either direction ------------------------------------------
+
+
+ASKED = {
+    "write k": lambda c, g: paged.kv_write(c, g(rows()), rows(), SLOTS),
+    "write v": lambda c, g: paged.kv_write(c, rows(), g(rows()), SLOTS),
+    "rope q": lambda c, g: rope(c, q_in=g(rows(heads=4).flatten(1))),
+    "rope k": lambda c, g: rope(c, k_in=g(rows().flatten(1))),
+    "rope v": lambda c, g: rope(c, v_in=g(rows().flatten(1))),
+    "rope cos": lambda c, g: rope(c, cos=g(torch.zeros(8, 32))),
+    "rope sin": lambda c, g: rope(c, sin=g(torch.zeros(8, 32))),
+    "attend q": lambda c, g: attend(c, g(rows(heads=4))),
+    "attend out": lambda c, g: attend(c, out=g(rows(heads=4))),
+    "attend cache": lambda c, g: attend(paged.PagedKVCache(c.k, g(c.v))),
+    "read cache": lambda c, g: paged.kv_read(
+        paged.PagedKVCache(g(c.k), c.v), SLOTS),
+    "write cache": lambda c, g: paged.kv_write(
+        paged.PagedKVCache(g(c.k), c.v), rows(), rows(), SLOTS),
+}
+
+
+@pytest.mark.parametrize("call", ASKED.values(), ids=ASKED.keys())
+def test_no_gradient_in_either_direction(call):
+    def leaf(x):
+        return x.detach().requires_grad_()
+
+    with pytest.raises(RuntimeError, match="no backward"):
+        call(cache(), leaf)
+    with torch.no_grad(), pytest.raises(ValueError, match="run on a GPU"):
+        call(cache(), leaf)
+    with fw.dual_level():
+        def dual(x):
+            return fw.make_dual(x.detach(), torch.ones_like(x))
+
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(cache(), dual)
+        # no_grad does not end forward mode
+        with torch.no_grad(), pytest.raises(RuntimeError,
+                                            match="no backward"):
+            call(cache(), dual)
