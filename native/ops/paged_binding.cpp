@@ -129,6 +129,10 @@ bool aligned(const Tensor& t) {
 
 void check_pools(Pools& p) {
   const Tensor &k = p.k, &v = p.v;
+  check_plain("k", k);
+  check_plain("v", v);
+  if (p.k_scale.defined()) check_plain("k_scale", p.k_scale);
+  if (p.v_scale.defined()) check_plain("v_scale", p.v_scale);
   if (k.dim() != 4 || k.sizes() != v.sizes())
     refuse("k and v pools are [pages, kv_heads, page_size, head_dim], of one "
            "shape: got ", shape(k), " and ", shape(v));
@@ -169,9 +173,12 @@ void check_pools(Pools& p) {
   p.device = k.device();
 }
 
+// looked at again at every call: a tensor can be resized, or given other memory
 const Pools& pools_of(PyObject* o) {
   if (!PyObject_TypeCheck(o, pools_type)) refuse("a PagedKVCache is wanted");
-  return reinterpret_cast<PoolsObject*>(o)->p;
+  Pools& p = reinterpret_cast<PoolsObject*>(o)->p;
+  check_pools(p);
+  return p;
 }
 
 // ---- what the operators ask of their arguments --------------------------------

@@ -174,3 +174,42 @@ def test_no_gradient_in_either_direction(call):
         with torch.no_grad(), pytest.raises(RuntimeError,
                                             match="no backward"):
             call(cache(), dual)
+
+
+# ---- a cache whose tensors were changed under it ----------------------------
+
+
+@pytest.mark.parametrize("change,match", [
+    (lambda x: x.resize_(1, 2, 16, 64), "of one shape"),
+    (lambda x: x.set_(torch.zeros(5, 2, 16, 32, dtype=BF16)), "of one shape"),
+    (lambda x: x.swapaxes_(1, 2), "of one shape"),
+    (lambda x: setattr(x, "data", torch.zeros(5, 2, 16, 64)), "bfloat16"),
+    (lambda x: setattr(x, "data", torch.zeros(5, 2, 64, 16, dtype=BF16).mT),
+     "without gaps"),
+    (lambda x: setattr(x, "data", torch.zeros(5 * 2 * 16 * 64 + 1, dtype=BF16)
+                       [1:].view(5, 2, 16, 64)), "multiples of 16"),
+    (lambda x: x.untyped_storage().resize_(0), "plain tensor"),
+    (lambda x: x.untyped_storage().resize_(4096), "plain tensor"),
+], ids=["resize", "set", "swapaxes", "type", "gaps", "address", "emptied",
+        "cut"])
+def test_a_cache_that_was_changed(change, match):
+    """What is read is what the tensors are at the call."""
+
+    for which in "kv":
+        c = cache()
+        change(getattr(c, which))
+        for call in (lambda: paged.kv_write(c, rows(), rows(), SLOTS),
+                     lambda: paged.kv_read(c, SLOTS), lambda: rope(c),
+                     lambda: attend(c)):
+            with pytest.raises(ValueError, match=match):
+                call()
+
+
+def test_a_cache_that_was_moved():
+    """Other memory of the same kind is taken as it is."""
+
+    c = cache()
+    for x in (c.k, c.v):
+        x.data = torch.zeros(9, 2, 16, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="run on a GPU"):
+        attend(c)
