@@ -260,6 +260,14 @@ void launched(const char* name, int rc) {
                              std::to_string(rc));
 }
 
+// of less than 2^32 lanes in all, in workgroups of 256
+constexpr int64_t LAUNCH = 1LL << 24;
+
+// rows of the cache, at 2048 / D a workgroup
+void check_count(const Pools& p, int64_t n) {
+  if (n > (LAUNCH - 1) * (2048 / p.D)) refuse("too many rows (", n, ")");
+}
+
 void write(const Pools& p, const Tensor& q, const Tensor& k, const Tensor& v,
            int64_t k_head, int64_t v_head, const Tensor& cos,
            const Tensor& sin, const Tensor& pos, const Tensor& slots,
@@ -281,9 +289,9 @@ void kv_write(const Pools& p, Tensor k, Tensor v, const Tensor& slots) {
     refuse("k and v are ", Shape{want}, ": got ", shape(k), " and ", shape(v));
   check_rows(p, {&k, &v});
   check_index("slots", slots, n);
+  check_count(p, n);
   no_grad({&k, &v, &p.k, &p.v});
   on_gpu(p, {&k, &v, &slots});
-  if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   if (n == 0) return;
   const c10::DeviceGuard guard(p.device);
   k = source_of(p, k);
@@ -312,8 +320,8 @@ Tensor rope_kv_write(const Pools& p, Tensor q_in, Tensor k_in, Tensor v_in,
       refuse("cos and sin are float32 [positions, ", D / 2, "] without gaps");
   check_index("pos", pos, n);
   check_index("slots", slots, n);
-  if (heads + 2 * p.kv_heads > 65535 || n >= (1LL << 31))
-    refuse("too many heads (", heads, ") or rows (", n, ")");
+  if (heads + 2 * p.kv_heads > 65535) refuse("too many heads (", heads, ")");
+  check_count(p, n);
   no_grad({&q_in, &k_in, &v_in, &cos, &sin, &p.k, &p.v});
   on_gpu(p, {&q_in, &k_in, &v_in, &cos, &sin, &pos, &slots});
   const c10::DeviceGuard guard(p.device);
@@ -335,9 +343,9 @@ std::pair<Tensor, Tensor> kv_read(const Pools& p, const Tensor& slots,
   if (slots.dim() != 1) refuse("slots is int64 [n]: got ", shape(slots));
   const int64_t n = slots.size(0);
   check_index("slots", slots, n);
+  check_count(p, n);
   no_grad({&p.k, &p.v});
   on_gpu(p, {&slots});
-  if (n >= (1LL << 31)) refuse("too many rows (", n, ")");
   const c10::DeviceGuard guard(p.device);
   const auto options = p.k.options().dtype(dtype);
   Tensor k = fresh(at::empty({n, p.kv_heads, p.D}, options));
@@ -460,6 +468,16 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
   if (Hq > 32768 || T >= most || B >= most || T * G + 128 * B >= most ||
       (T * G / 16 + B) * Hk >= most)
     refuse(T, " tokens of ", Hq, " heads: too many for a launch");
+  Plan plan{0, 4, 0, 1};
+  if (T && B) {
+    plan = plan_of(T, B, G, Hk, D, cols << p.page_log2, p.quantized);
+    // shared, an item has at least 5 of the line's 2^30 units, and one to spare
+    const int64_t items = (T * G / (plan.workers ? 16 : 128) + B) * Hk;
+    if (plan.join ? items > (1LL << 30) / 6
+                  : items * plan.splits > LAUNCH - 8)
+      refuse(B, " sequences, ", T, " tokens of ", Hq, " heads: too many for a "
+             "launch");
+  }
   if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)D);
   no_grad({&q, &out, &p.k, &p.v});
   if (out.defined()) {
@@ -480,7 +498,6 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
   // several workgroups may read a row that one of them answers
   q = overlap(out, q) ? fresh(q.clone(at::MemoryFormat::Contiguous))
                       : rows_of(q);
-  const Plan plan = plan_of(T, B, G, Hk, D, cols << p.page_log2, p.quantized);
   Tensor parts;
   if (plan.join || plan.splits > 1) {
     // its own for every call: two captured graphs never share it

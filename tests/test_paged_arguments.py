@@ -213,3 +213,42 @@ def test_a_cache_that_was_moved():
         x.data = torch.zeros(9, 2, 16, 64, dtype=BF16)
     with pytest.raises(ValueError, match="run on a GPU"):
         attend(c)
+
+
+# ---- more than one launch takes ---------------------------------------------
+
+
+def steps(B, heads, cols=1):
+    """B steps over as many heads, without memory of that size."""
+
+    c = paged.make_cache(1, 16, heads, 32, device="cpu")
+    return paged.paged_attention(
+        torch.zeros(1, 1, 32, dtype=BF16).expand(B, heads, 32), c,
+        torch.zeros(B + 1, dtype=I32), torch.zeros(B, dtype=I32),
+        torch.zeros(cols, dtype=I32).expand(B, cols))
+
+
+def test_more_than_a_launch_takes():
+    """A launch has less than 2**32 lanes, 2**24 workgroups of 256: here one
+    for each of the B + B / 16 places of tiles, and head. Shared out by
+    length, the places for tiles have 5 numbers each at least, of 2**30."""
+
+    for fits, cols in ((493447, 1), (5263440, 1024)):
+        with pytest.raises(ValueError, match="run on a GPU"):
+            steps(fits, 32, cols)
+        with pytest.raises(ValueError, match="too many"):
+            steps(fits + 1, 32, cols)
+    row = torch.zeros(1, 1, 1, dtype=BF16)
+    c = paged.make_cache(1, 16, 1, 128, device="cpu")
+    n = 2 ** 28  # 16 a workgroup
+    k = row.expand(n, 1, 128)
+    huge = torch.empty(n, dtype=torch.int64)  # never touched
+    with pytest.raises(ValueError, match="run on a GPU"):
+        paged.kv_write(c, k[16:], k[16:], huge[16:])
+    for call in (lambda: paged.kv_write(c, k, k, huge),
+                 lambda: paged.kv_read(c, huge),
+                 lambda: paged.rope_kv_write(
+                     c, k[:, 0], k[:, 0], k[:, 0], torch.zeros(1, 64),
+                     torch.zeros(1, 64), huge, huge, 1)):
+        with pytest.raises(ValueError, match="too many"):
+            call()
