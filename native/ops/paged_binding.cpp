@@ -268,6 +268,11 @@ void check_count(const Pools& p, int64_t n) {
   if (n > (LAUNCH - 1) * (2048 / p.D)) refuse("too many rows (", n, ")");
 }
 
+// written in place: autograd notices where it had kept the values
+void changed(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void write(const Pools& p, const Tensor& q, const Tensor& k, const Tensor& v,
            int64_t k_head, int64_t v_head, const Tensor& cos,
            const Tensor& sin, const Tensor& pos, const Tensor& slots,
@@ -280,6 +285,7 @@ void write(const Pools& p, const Tensor& q, const Tensor& k, const Tensor& v,
                ptr(q_out), ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale),
                p.pages, p.page_log2, n, heads, p.kv_heads, p.D,
                k.scalar_type() == at::kHalf, stream_of(p)));
+  for (const Tensor* t : {&p.k, &p.v, &p.k_scale, &p.v_scale}) changed(*t);
 }
 
 void kv_write(const Pools& p, Tensor k, Tensor v, const Tensor& slots) {
@@ -516,6 +522,7 @@ Tensor attention(const Pools& p, Tensor q, const Tensor& starts,
                (float)scale, causal, q.scalar_type() == at::kHalf,
                (int)plan.workers, (int)plan.waves, (int)plan.join, (int)plan.splits,
                stream_of(p)));
+  changed(out);
   return out;
 }
 

@@ -107,3 +107,46 @@ def test_rope_rows_of_the_cache():
     assert torch.equal(*outs)
     for a, b in zip(paged.kv_read(apart, slots), paged.kv_read(over, slots)):
         assert torch.equal(a, b)
+
+
+# ---- what autograd has kept ---------------------------------------------------
+
+
+def test_a_tensor_kept_for_a_backward_pass_is_missed():
+    """What is written in place counts as changed: a backward pass that had
+    kept it is refused, and not computed from what lies there now."""
+
+    b = Batch([(1, 40), (2, 30)], 4, 2, 64, 16, BF16, True, seed=1)
+    q, starts = b.q.cuda(), b.q_starts.cuda()
+    lens, table = b.kv_lens.cuda(), b.table.cuda()
+    out, w = torch.zeros_like(q), torch.ones_like(q, requires_grad=True)
+    y = (out * w).sum()
+    paged.paged_attention(q, b.cache, starts, lens, table, out=out)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    c, slots = b.cache, torch.arange(3, device="cuda")
+    k = torch.randn(3, 2, 64, device="cuda").to(BF16)
+    cos = torch.ones(3, 32, device="cuda")
+    kept = [c.k, c.v, c.k_scale, c.v_scale]
+    for write in (lambda: paged.kv_write(c, k, k, slots),
+                  lambda: paged.rope_kv_write(
+                      c, k.flatten(1), k.flatten(1), k.flatten(1), cos, cos,
+                      slots, slots, 2)):
+        before = [x._version for x in kept]
+        write()
+        assert all(x._version > v for x, v in zip(kept, before))
+    before = [x._version for x in kept]
+    paged.kv_read(c, slots)
+    paged.paged_attention(q, c, starts, lens, table)
+    assert [x._version for x in kept] == before
+
+
+def test_under_inference_mode():
+    with torch.inference_mode():
+        b = Batch([(1, 40), (2, 30)], 4, 2, 64, 16, BF16, False, seed=1)
+        out = torch.empty(3, 4, 64, dtype=BF16, device="cuda")
+        check(b.run(out=out), *b.want())
+        k = torch.randn(3, 2, 64, device="cuda").to(BF16)
+        slots = torch.arange(3, device="cuda")
+        paged.kv_write(b.cache, k, k, slots)
+        assert torch.equal(paged.kv_read(b.cache, slots)[0], k)
