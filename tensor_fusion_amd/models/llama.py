@@ -110,7 +110,81 @@ def paged_caches(layers: int, pages: int, page_size: int, kv_heads: int,
                              quantized, device) for _ in range(layers)]
 
 
-class Attention(nn.Module):
+class Relaid:
+    """The weights of some layers in another layout, merged or shuffled for
+    the decode products, for as long as they are what was laid out.
+
+    A weight that was changed in place, loaded, converted, moved or replaced
+    is laid out again, in the same memory where that fits: a captured graph
+    may read it. Writes through `weight.data` are none that torch counts, and
+    are not seen; nor are those to weights made under torch.inference_mode(),
+    but for loading and converting the model."""
+
+    def __init__(self, lay):
+        self.lay, self.value, self.of = lay, None, ()
+
+    def get(self, *layers):
+        # no attributes of modules, which are slow: this is for each layer
+        # of a decode step
+        for lin, (of, w, _, version, at) in zip(layers, self.of):
+            if (lin is not of or lin._parameters.get("weight") is not w
+                    or w.data_ptr() != at
+                    or version is not None and w._version != version):
+                break
+        else:
+            if self.of:
+                return self.value
+        return self._lay(layers)
+
+    def _lay(self, layers):
+        ws = [lin.weight for lin in layers]
+        with torch.inference_mode(False), torch.no_grad():
+            value = self.lay(*(w.detach() for w in ws))
+            if any(lin._parameters.get("weight") is not w
+                   for lin, w in zip(layers, ws)):
+                return value  # worked out anew at every call, as they are
+            if value.is_cuda and torch.cuda.is_current_stream_capturing():
+                return value  # there from the replay on only
+            old = self.value
+            if old is not None and (old.shape, old.dtype, old.device) == (
+                    value.shape, value.dtype, value.device):
+                value = old.copy_(value)
+        self.value = value
+        # the alias keeps the address from being another weight's
+        self.of = [(lin, w, w.detach(),
+                    None if w.is_inference() else w._version, w.data_ptr())
+                   for lin, w in zip(layers, ws)]
+        return value
+
+
+def merged(*weights):
+    return torch.cat(weights)
+
+
+def packed(weight):
+    from ..ops import fused
+    return fused.pack_skinny_weight(weight)
+
+
+class KeepsLayouts(nn.Module):
+    """A module with Relaid weights: loading and converting forgets them."""
+
+    def _forget(self):
+        for x in self.__dict__.values():
+            for r in x.values() if isinstance(x, dict) else (x,):
+                if isinstance(r, Relaid):
+                    r.of = ()
+
+    def _apply(self, *args, **kw):
+        self._forget()
+        return super()._apply(*args, **kw)
+
+    def _load_from_state_dict(self, *args, **kw):
+        self._forget()
+        return super()._load_from_state_dict(*args, **kw)
+
+
+class Attention(KeepsLayouts):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.cfg = cfg
@@ -119,8 +193,8 @@ class Attention(nn.Module):
         self.wk = nn.Linear(cfg.dim, cfg.kv_heads * self.head_dim, bias=False)
         self.wv = nn.Linear(cfg.dim, cfg.kv_heads * self.head_dim, bias=False)
         self.wo = nn.Linear(cfg.heads * self.head_dim, cfg.dim, bias=False)
-        self._packed = None  # decode-GEMV weight shuffles (lazy)
-        self._wqkv = None    # merged qkv weight (fused path, lazy)
+        self._packed = {}  # decode-GEMV weight shuffles
+        self._wqkv = Relaid(merged)  # fused path
 
     def _proj(self, lin: nn.Linear, x, idx: int):
         """Decode projections via the packed MFMA GEMV when the token
@@ -135,12 +209,7 @@ class Attention(nn.Module):
         from ..ops import fused
         if not fused.packed_profitable(lin.out_features, D):
             return lin(x)
-        if self._packed is None:
-            self._packed = {}
-        wp = self._packed.get(idx)
-        if wp is None:
-            wp = fused.pack_skinny_weight(lin.weight.detach())
-            self._packed[idx] = wp
+        wp = self._packed.setdefault(idx, Relaid(packed)).get(lin)
         flat = x.reshape(B * T, D)
         if not flat.is_contiguous():
             flat = flat.contiguous()
@@ -150,12 +219,10 @@ class Attention(nn.Module):
         """q, k and v as columns of ONE product (decode is weight
         streaming: 3 launches -> 1)."""
 
-        if self._wqkv is None:
-            self._wqkv = torch.cat(
-                [self.wq.weight, self.wk.weight, self.wv.weight],
-                dim=0).detach().contiguous()
+        m = self._modules
+        w = self._wqkv.get(m["wq"], m["wk"], m["wv"])
         dk = self.cfg.kv_heads * self.head_dim
-        return F.linear(x, self._wqkv).split(
+        return F.linear(x, w).split(
             [self.cfg.heads * self.head_dim, dk, dk], dim=-1)
 
     def _paged(self, x, cos, sin, cache, batch):
@@ -248,14 +315,14 @@ class Attention(nn.Module):
         return self._proj(self.wo, o, 3)
 
 
-class MLP(nn.Module):
+class MLP(KeepsLayouts):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.gate = nn.Linear(cfg.dim, cfg.intermediate, bias=False)
         self.up = nn.Linear(cfg.dim, cfg.intermediate, bias=False)
         self.down = nn.Linear(cfg.intermediate, cfg.dim, bias=False)
-        self._packed = None
-        self._wgu = None  # merged gate+up weight (fused path, lazy)
+        self._packed = {}
+        self._wgu = Relaid(merged)  # gate and up, fused path
 
     _proj = Attention._proj  # same packed-GEMV decode routing
 
@@ -265,11 +332,8 @@ class MLP(nn.Module):
             # gate+up = ONE merged GEMM, then one silu*mul kernel over
             # the two column halves
             from ..ops import fused
-            if self._wgu is None:
-                self._wgu = torch.cat(
-                    [self.gate.weight, self.up.weight],
-                    dim=0).detach().contiguous()
-            gu = F.linear(x, self._wgu)
+            m = self._modules
+            gu = F.linear(x, self._wgu.get(m["gate"], m["up"]))
             h = fused.silu_mul_gu(gu, self.gate.out_features)
             return self._proj(self.down, h, 2)
         g = self._proj(self.gate, x, 0)
@@ -293,7 +357,7 @@ class Block(nn.Module):
         return x
 
 
-class Llama(nn.Module):
+class Llama(KeepsLayouts):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.cfg = cfg
@@ -301,6 +365,7 @@ class Llama(nn.Module):
         self.blocks = nn.ModuleList(Block(cfg) for _ in range(cfg.layers))
         self.norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.lm_head = nn.Linear(cfg.dim, cfg.vocab, bias=False)
+        self._lm_packed = Relaid(packed)
 
     def forward(self, tokens, pos=None, caches=None, pos_end=None,
                 mask=None):
@@ -349,12 +414,10 @@ class Llama(nn.Module):
         B, T, D = normed.shape
         if (B * T <= 16 and D % 32 == 0
                 and self.lm_head.weight.shape[0] % 16 == 0):
-            if getattr(self, "_lm_packed", None) is None:
-                self._lm_packed = fused.pack_skinny_weight(
-                    self.lm_head.weight.detach())
             flat = normed.reshape(B * T, D).contiguous()
             out = fused.skinny_gemm_packed(
-                flat, self._lm_packed, self.lm_head.weight.shape[0])
+                flat, self._lm_packed.get(self.lm_head),
+                self.lm_head.weight.shape[0])
             return out.view(B, T, -1)
         return self.lm_head(normed)
 
