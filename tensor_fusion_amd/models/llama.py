@@ -230,9 +230,9 @@ class Attention(KeepsLayouts):
         ops/paged.py, for new tokens of any number of sequences."""
 
         from ..ops import paged
-        if _FUSED_OPS:
+        if _FUSED_OPS and not torch.is_grad_enabled():
             q, k, v = self._merged_qkv(x)
-        else:
+        else:  # a gradient that is asked for is refused further on
             q, k, v = self.wq(x), self.wk(x), self.wv(x)
         o = paged.attend(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1),
                          cos, sin, cache, batch, self.cfg.heads)

@@ -9,6 +9,8 @@ import torch.nn.functional as F
 
 from tensor_fusion_amd.models import llama as L
 
+pytestmark = pytest.mark.usefixtures("native_built")
+
 
 def attention(dtype=torch.float32, seed=0):
     torch.manual_seed(seed)
@@ -99,3 +101,30 @@ def test_weights_made_under_inference_mode():
         a._merged_qkv(x.double())
     with torch.no_grad():
         a._merged_qkv(x.double())
+
+
+def test_merged_weights_ask_for_gradients():
+    """Over pages too: a weight that asks for a gradient is not served from a
+    copy that does not."""
+
+    from tensor_fusion_amd.ops import paged
+    a = attention(torch.bfloat16)
+    cache = paged.make_cache(4, 16, 2, 32, device="cpu")
+    batch = paged.PagedBatch.of(torch.zeros(1, 4, dtype=torch.int32),
+                                torch.zeros(1, dtype=torch.int64), 3, 16)
+    t = torch.zeros(8, 16)
+    x = torch.zeros(1, 3, 128, dtype=torch.bfloat16)
+    fused, L._FUSED_OPS = L._FUSED_OPS, True
+    try:
+        with pytest.raises(ValueError, match="run on a GPU"):
+            a(x, t, t, batch.pos, (cache, batch))
+        for w in (a.wq.weight, a.wk.weight, a.wv.weight):
+            w.requires_grad_()
+            with pytest.raises(RuntimeError, match="no backward"):
+                a(x, t, t, batch.pos, (cache, batch))
+            with torch.no_grad(), pytest.raises(ValueError,
+                                                match="run on a GPU"):
+                a(x, t, t, batch.pos, (cache, batch))
+            w.requires_grad_(False)
+    finally:
+        L._FUSED_OPS = fused
