@@ -136,13 +136,16 @@ def make_cache(pages: int, page_size: int, kv_heads: int, head_dim: int,
 class PagedBatch:
     """New tokens of some sequences, as the operators take them: packed one
     sequence after the other, token i at position pos[i] of its sequence, in
-    slot slots[i]; kv_lens counts them."""
+    slot slots[i]; kv_lens counts them. page_size is the one that the slots
+    were worked out for, and has to be the caches'; None where they are a
+    caller's own."""
 
     q_starts: torch.Tensor      # int32 [B + 1]
     kv_lens: torch.Tensor       # int32 [B]
     block_table: torch.Tensor   # int32 [B, columns]
     pos: torch.Tensor           # int64 [tokens]
     slots: torch.Tensor         # int64 [tokens]
+    page_size: int | None = None
 
     @classmethod
     def of(cls, block_table, past, new, page_size: int) -> "PagedBatch":
@@ -151,6 +154,8 @@ class PagedBatch:
         a number everything is worked out on the device, so that a step that
         is captured goes on from wherever `past` stands at the replay."""
 
+        if page_size < 1:
+            raise ValueError(f"no page_size of {page_size}")
         (B, cols), device = block_table.shape, block_table.device
         past = past.to(torch.int64)
         if isinstance(new, int):
@@ -180,12 +185,21 @@ class PagedBatch:
         page = block_table[seq, col.clamp(0, max(cols - 1, 0))]
         slots = page.to(torch.int64) * page_size + pos % page_size
         slots = torch.where(there, slots, -1)
-        return cls(starts, lens.to(torch.int32), block_table, pos, slots)
+        return cls(starts, lens.to(torch.int32), block_table, pos, slots,
+                   page_size)
+
+    def check(self, cache: PagedKVCache) -> None:
+        if self.page_size is not None and self.page_size != cache.page_size:
+            raise ValueError(f"a batch for pages of {self.page_size} tokens, "
+                             f"and a cache with pages of {cache.page_size}")
 
     def over(self, caches):
         """The layers' caches, as a model takes them with this batch."""
 
-        return [(c, self) for c in caches]
+        layers = [(c, self) for c in caches]
+        for c, _ in layers:
+            self.check(c)
+        return layers
 
 
 def attend(q_in, k_in, v_in, cos, sin, cache: PagedKVCache,
@@ -193,6 +207,7 @@ def attend(q_in, k_in, v_in, cos, sin, cache: PagedKVCache,
     """A layer's attention between its projections: rope_kv_write, then
     paged_attention. Returns [tokens, heads * head_dim]."""
 
+    batch.check(cache)
     q = rope_kv_write(cache, q_in, k_in, v_in, cos, sin, batch.pos,
                       batch.slots, heads)
     out = paged_attention(q, cache, batch.q_starts, batch.kv_lens,

@@ -252,3 +252,38 @@ def test_more_than_a_launch_takes():
                      torch.zeros(1, 64), huge, huge, 1)):
         with pytest.raises(ValueError, match="too many"):
             call()
+
+
+# ---- a batch for pages of another size ----------------------------------------
+
+
+def batch_of(page, new=3):
+    return paged.PagedBatch.of(torch.zeros(1, 4, dtype=I32),
+                               torch.zeros(1, dtype=torch.int64), new, page)
+
+
+def test_a_batch_of_another_page_size():
+    """Its slots would lie in pages of other sequences."""
+
+    c, t = cache(), torch.zeros(8, 32)
+    q, k = rows(heads=4).flatten(1), rows().flatten(1)
+    for new in (3, [3]):
+        for page in (8, 32, 64):
+            b = batch_of(page, new)
+            assert b.page_size == page
+            with pytest.raises(ValueError, match="pages of"):
+                paged.attend(q, k, k, t, t, c, b, 4)
+            with pytest.raises(ValueError, match="pages of"):
+                b.over([c])
+        b = batch_of(16, new)
+        with pytest.raises(ValueError, match="run on a GPU"):
+            paged.attend(q, k, k, t, t, c, b, 4)
+        assert [*map(id, sum(b.over(iter([c, c])), ()))] == [id(c), id(b)] * 2
+    # slots of a caller's own
+    own = paged.PagedBatch(b.q_starts, b.kv_lens, b.block_table, b.pos,
+                           b.slots)
+    with pytest.raises(ValueError, match="run on a GPU"):
+        paged.attend(q, k, k, t, t, c, own, 4)
+    for page in (0, -16):
+        with pytest.raises(ValueError, match="page_size"):
+            batch_of(page)
