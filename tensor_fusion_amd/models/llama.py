@@ -93,14 +93,19 @@ def apply_rope(x, cos, sin, pos):
     return out
 
 
-def is_paged(cache) -> bool:
+def is_paged(cache, mask=None) -> bool:
     """Whether a layer's cache is (PagedKVCache, PagedBatch), as
-    PagedBatch.over gives it."""
+    PagedBatch.over gives it. Its attention takes no mask."""
 
     if cache is None or isinstance(cache[0], torch.Tensor):
         return False
     from ..ops import paged
-    return isinstance(cache[0], paged.PagedKVCache)
+    if not isinstance(cache[0], paged.PagedKVCache):
+        return False
+    if mask is not None:
+        raise ValueError("attention over a paged cache takes no mask: it sees "
+                         "the keys that the batch's lengths count")
+    return True
 
 
 def paged_caches(layers: int, pages: int, page_size: int, kv_heads: int,
@@ -242,7 +247,7 @@ class Attention(KeepsLayouts):
                 mask=None):
         B, T, _ = x.shape
         cfg = self.cfg
-        if is_paged(cache):
+        if is_paged(cache, mask):
             return self._paged(x, cos, sin, *cache)
         if (_FUSED_OPS and x.is_cuda and x.dtype == torch.bfloat16
                 and cache is not None and self.head_dim % 8 == 0

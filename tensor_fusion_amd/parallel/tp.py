@@ -85,7 +85,7 @@ class TPAttention(nn.Module):
     def forward(self, x, cos, sin, pos, cache=None, pos_end=None,
                 mask=None):
         B, T, _ = x.shape
-        if is_paged(cache):
+        if is_paged(cache, mask):
             from ..ops import paged
             o = paged.attend(*(w(x).flatten(0, 1) for w in (self.wq, self.wk,
                                                             self.wv)),

@@ -128,3 +128,22 @@ def test_merged_weights_ask_for_gradients():
             w.requires_grad_(False)
     finally:
         L._FUSED_OPS = fused
+
+
+def test_a_mask_over_pages():
+    """Attention over pages takes none: it is not passed over."""
+
+    from tensor_fusion_amd.ops import paged
+    from tensor_fusion_amd.parallel.tp import TPAttention
+    cfg = L.CONFIGS["tiny"]
+    cache = paged.make_cache(4, 16, 2, 32, device="cpu")
+    batch = paged.PagedBatch.of(torch.zeros(1, 4, dtype=torch.int32),
+                                torch.zeros(1, dtype=torch.int64), 3, 16)
+    t, x = torch.zeros(8, 16), torch.zeros(1, 3, 128, dtype=torch.bfloat16)
+    for a in (attention(torch.bfloat16),
+              TPAttention(cfg, 1).bfloat16().requires_grad_(False)):
+        with pytest.raises(ValueError, match="mask"):
+            a(x, t, t, batch.pos, (cache, batch),
+              mask=torch.zeros(1, 1, 1, 64))
+        with pytest.raises(ValueError, match="run on a GPU"):
+            a(x, t, t, batch.pos, (cache, batch))
