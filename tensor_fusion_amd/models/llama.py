@@ -569,6 +569,9 @@ def decode_bench_paged(model: Llama, batch: int, ctx: int, steps: int,
     from ..ops.paged import PagedBatch
     cfg = model.cfg
     warmup = max(warmup, 1)
+    last = ctx + steps + warmup + (3 if graphs else 0)
+    if last > cfg.max_seq:
+        raise ValueError(f"{last} positions for a model of {cfg.max_seq}")
     width = -(-(ctx + steps + warmup + 8) // page_size)
     caches = model.make_paged_cache(batch * width, page_size, device, dtype,
                                     quantized)

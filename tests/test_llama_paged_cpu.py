@@ -1,5 +1,5 @@
-"""The merged and shuffled copies of weights that the fused path keeps: they
-follow the weights."""
+"""The merged and shuffled copies of weights that the fused path keeps, which
+follow the weights; and what the models refuse over pages. No GPU needed."""
 import copy
 
 import pytest
@@ -147,3 +147,18 @@ def test_a_mask_over_pages():
               mask=torch.zeros(1, 1, 1, 64))
         with pytest.raises(ValueError, match="run on a GPU"):
             a(x, t, t, batch.pos, (cache, batch))
+
+
+def test_a_decode_benchmark_past_the_positions():
+    """Rows past the rotation's tables are NaN: no time is given for them."""
+
+    m = L.build_model("tiny", device="cpu")
+    for graphs, most in ((False, 512 - 12), (True, 512 - 15)):
+        def run(ctx):
+            L.decode_bench_paged(m, 1, ctx, 10, 2, graphs=graphs,
+                                 device="cpu")
+
+        with pytest.raises(ValueError, match="run on a GPU"):
+            run(most)
+        with pytest.raises(ValueError, match="positions"):
+            run(most + 1)
