@@ -243,10 +243,13 @@ def build_all(only=None, force=False):
     global FORCE
     FORCE = force
     results = {}
-    for name, fn in ALL.items():
-        if only and name != only:
-            continue
-        results[name] = fn()
+    try:
+        for name, fn in ALL.items():
+            if only and name != only:
+                continue
+            results[name] = fn()
+    finally:
+        FORCE = False
     return results
 
 
