@@ -1,4 +1,6 @@
 """The build script's own behaviour: nothing is compiled here."""
+import sys
+
 import pytest
 
 import build_native
@@ -16,3 +18,12 @@ def test_force_ends_with_its_call(monkeypatch):
     assert not build_native.FORCE
     build_native.build_all("one")
     assert seen == [True, False]
+
+
+def test_without_torch_the_binding_is_left_out(monkeypatch, capsys):
+    """Everything else needs compilers only, and is built without it."""
+
+    monkeypatch.setitem(sys.modules, "torch", None)
+    monkeypatch.setattr(build_native, "_run", lambda cmd: pytest.fail(str(cmd)))
+    assert build_native.build_paged_binding() is None
+    assert "torch" in capsys.readouterr().out
