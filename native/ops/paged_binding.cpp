@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <new>
 #include <sstream>
@@ -649,18 +650,38 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// sizes of a batch: T, B, G, Hk, D and the table's keys
+std::array<int64_t, 6> sizes_of(PyObject* const* a) {
+  std::array<int64_t, 6> x;
+  for (int i = 0; i < 6; ++i) {
+    x[i] = int_of(a[i], "a size");
+    if (x[i] < (i < 5) || x[i] > (i < 5 ? 1LL << 18 : 1LL << 30))
+      refuse("no plan for a size of ", x[i]);
+  }
+  return x;
+}
+
+// of a 16-bit cache: workers, join, splits
 PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     count(n, 6);
-    int64_t x[6];
-    for (int i = 0; i < 6; ++i) {
-      x[i] = int_of(a[i], "a size");
-      if (x[i] < (i < 5) || x[i] > (i < 5 ? 1LL << 18 : 1LL << 30))
-        refuse("no plan for a size of ", x[i]);
-    }
+    const auto x = sizes_of(a);
     const Plan p = plan_of(x[0], x[1], x[2], x[3], x[4], x[5], false);
     return Py_BuildValue("LLL", (long long)p.workers, (long long)p.join,
                          (long long)p.splits);
+  });
+}
+
+// of either cache: workers, waves, join, splits
+PyObject* py_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 7);
+    const auto x = sizes_of(a);
+    const int quantized = PyObject_IsTrue(a[6]);
+    if (quantized < 0) return nullptr;
+    const Plan p = plan_of(x[0], x[1], x[2], x[3], x[4], x[5], quantized);
+    return Py_BuildValue("LLLL", (long long)p.workers, (long long)p.waves,
+                         (long long)p.join, (long long)p.splits);
   });
 }
 
@@ -672,6 +693,7 @@ PyMethodDef methods[] = {
     {"kv_read", TF_FAST(py_kv_read), METH_FASTCALL, nullptr},
     {"attention", TF_FAST(py_attention), METH_FASTCALL, nullptr},
     {"plan", TF_FAST(py_plan), METH_FASTCALL, nullptr},
+    {"dispatch", TF_FAST(py_dispatch), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tf_paged", nullptr, -1, methods,
