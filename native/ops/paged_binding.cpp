@@ -9,7 +9,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGuard.h>
@@ -92,6 +91,14 @@ PyTypeObject* pools_type = nullptr;
 
 bool wide(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 
+// bytes from the first value to the end of the last one; t has values
+size_t extent(const Tensor& t) {
+  const auto sizes = t.sizes(), strides = t.strides();
+  int64_t last = 0;
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+  return (last + 1) * t.itemsize();
+}
+
 // A kernel is given addresses: what lies there has to be the tensor's values.
 // It is not where a Python class or a function transform stands between (fake,
 // distributed and batched tensors), where a sign is still to be applied, or
@@ -105,9 +112,8 @@ void check_plain(const char* name, const Tensor& t) {
        DispatchKey::Conjugate});
   if (t.layout() != at::kStrided || t.is_nested() ||
       t.key_set().has_any(between) ||
-      (t.numel() && at::detail::computeStorageNbytes(
-                        t.sizes(), t.strides(), t.itemsize(),
-                        t.storage_offset()) > t.storage().nbytes()))
+      (t.numel() && t.storage_offset() * t.itemsize() + extent(t) >
+                        t.storage().nbytes()))
     refuse(name, " is a plain tensor: dense, with its values in its memory");
 }
 
@@ -234,11 +240,7 @@ bool overlap(const Tensor& a, const Tensor& b) {
   auto at = [](const Tensor& t) {
     return reinterpret_cast<uintptr_t>(t.data_ptr());
   };
-  auto bytes = [](const Tensor& t) {
-    return at::detail::computeStorageNbytes(t.sizes(), t.strides(),
-                                            t.itemsize());
-  };
-  return at(a) < at(b) + bytes(b) && at(b) < at(a) + bytes(a);
+  return at(a) < at(b) + extent(b) && at(b) < at(a) + extent(a);
 }
 
 // rows to be written, and not from under them: rows that lie in the cache are
