@@ -22,6 +22,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import fused, paged
+
 
 @dataclass
 class LlamaConfig:
@@ -63,7 +65,6 @@ class RMSNorm(nn.Module):
                 and x.shape[-1] % 8 == 0 and x.is_contiguous()):
             # one gfx950 kernel instead of ~5 eager kernels (ops/fused.py;
             # numerics vs the fp32 reference: tests/test_gpu_fused.py)
-            from ..ops import fused
             return fused.rmsnorm(x, self.weight, self.eps)
         dt = x.dtype
         x = x.float()
@@ -97,10 +98,7 @@ def is_paged(cache, mask=None) -> bool:
     """Whether a layer's cache is (PagedKVCache, PagedBatch), as
     PagedBatch.over gives it. Its attention takes no mask."""
 
-    if cache is None or isinstance(cache[0], torch.Tensor):
-        return False
-    from ..ops import paged
-    if not isinstance(cache[0], paged.PagedKVCache):
+    if cache is None or not isinstance(cache[0], paged.PagedKVCache):
         return False
     if mask is not None:
         raise ValueError("attention over a paged cache takes no mask: it sees "
@@ -110,7 +108,6 @@ def is_paged(cache, mask=None) -> bool:
 
 def paged_caches(layers: int, pages: int, page_size: int, kv_heads: int,
                  head_dim: int, device, dtype, quantized: bool):
-    from ..ops import paged
     return [paged.make_cache(pages, page_size, kv_heads, head_dim, dtype,
                              quantized, device) for _ in range(layers)]
 
@@ -126,20 +123,23 @@ class Relaid:
     but for loading and converting the model."""
 
     def __init__(self, lay):
-        self.lay, self.value, self.of = lay, None, ()
+        self.lay, self.value = lay, None
+        self.layers, self.of = (), ()
 
     def get(self, *layers):
-        # no attributes of modules, which are slow: this is for each layer
-        # of a decode step
-        for lin, (of, w, _, version, at) in zip(layers, self.of):
-            if (lin is not of or lin._parameters.get("weight") is not w
-                    or w.data_ptr() != at
-                    or version is not None and w._version != version):
-                break
-        else:
-            if self.of:
+        # without the attributes of modules, which are slow: this is for each
+        # layer of a decode step
+        if layers == self.layers:
+            for params, w, version, at, _ in self.of:
+                if (params.get("weight") is not w or w.data_ptr() != at
+                        or version is not None and w._version != version):
+                    break
+            else:
                 return self.value
         return self._lay(layers)
+
+    def forget(self):
+        self.layers = self.of = ()
 
     def _lay(self, layers):
         ws = [lin.weight for lin in layers]
@@ -154,11 +154,11 @@ class Relaid:
             if old is not None and (old.shape, old.dtype, old.device) == (
                     value.shape, value.dtype, value.device):
                 value = old.copy_(value)
-        self.value = value
+        self.value, self.layers = value, layers
         # the alias keeps the address from being another weight's
-        self.of = [(lin, w, w.detach(),
-                    None if w.is_inference() else w._version, w.data_ptr())
-                   for lin, w in zip(layers, ws)]
+        self.of = [(lin._parameters, w,
+                    None if w.is_inference() else w._version, w.data_ptr(),
+                    w.detach()) for lin, w in zip(layers, ws)]
         return value
 
 
@@ -167,7 +167,6 @@ def merged(*weights):
 
 
 def packed(weight):
-    from ..ops import fused
     return fused.pack_skinny_weight(weight)
 
 
@@ -178,7 +177,7 @@ class KeepsLayouts(nn.Module):
         for x in self.__dict__.values():
             for r in x.values() if isinstance(x, dict) else (x,):
                 if isinstance(r, Relaid):
-                    r.of = ()
+                    r.forget()
 
     def _apply(self, *args, **kw):
         self._forget()
@@ -211,7 +210,6 @@ class Attention(KeepsLayouts):
                 and B * T <= 16 and D % 32 == 0
                 and lin.out_features % 16 == 0):
             return lin(x)
-        from ..ops import fused
         if not fused.packed_profitable(lin.out_features, D):
             return lin(x)
         wp = self._packed.setdefault(idx, Relaid(packed)).get(lin)
@@ -234,7 +232,6 @@ class Attention(KeepsLayouts):
         """Rotation, cache write and attention over pages: two kernels of
         ops/paged.py, for new tokens of any number of sequences."""
 
-        from ..ops import paged
         if _FUSED_OPS and not torch.is_grad_enabled():
             q, k, v = self._merged_qkv(x)
         else:  # a gradient that is asked for is refused further on
@@ -257,7 +254,6 @@ class Attention(KeepsLayouts):
             # profiles/pmc_ktrace_r02.md). qkv = ONE merged GEMM (3
             # launches -> 1; the rope kernel reads the column slices
             # with their row stride)
-            from ..ops import fused
             qin, kin, vin = self._merged_qkv(x)
             k_cache, v_cache = cache
             q = fused.rope_qkv_cache(qin, kin, vin, cos, sin, pos,
@@ -336,7 +332,6 @@ class MLP(KeepsLayouts):
                 and self.gate.out_features % 8 == 0):
             # gate+up = ONE merged GEMM, then one silu*mul kernel over
             # the two column halves
-            from ..ops import fused
             m = self._modules
             gu = F.linear(x, self._wgu.get(m["gate"], m["up"]))
             h = fused.silu_mul_gu(gu, self.gate.out_features)
@@ -394,7 +389,6 @@ class Llama(KeepsLayouts):
         and every add+RMSNorm pair is ONE gfx950 kernel (ops/fused.py) —
         the vLLM-style fusion of the decode hot path."""
 
-        from ..ops import fused
         res = x.contiguous()
         normed = fused.rmsnorm(res, self.blocks[0].ln1.weight,
                                self.blocks[0].ln1.eps)
@@ -566,7 +560,6 @@ def decode_bench_paged(model: Llama, batch: int, ctx: int, steps: int,
     step: positions, slots and lengths advance on the device, and attention
     reads the valid keys only."""
 
-    from ..ops.paged import PagedBatch
     cfg = model.cfg
     warmup = max(warmup, 1)
     last = ctx + steps + warmup + (3 if graphs else 0)
@@ -579,13 +572,13 @@ def decode_bench_paged(model: Llama, batch: int, ctx: int, steps: int,
                          dtype=torch.int32).view(batch, width)
     past = torch.zeros(batch, dtype=torch.int64, device=device)
     toks = torch.randint(0, cfg.vocab, (batch, ctx), device=device)
-    first = PagedBatch.of(table, past, ctx, page_size)
+    first = paged.PagedBatch.of(table, past, ctx, page_size)
     model(toks, pos=first.pos, caches=first.over(caches))
     past.add_(ctx)
     cur = torch.randint(0, cfg.vocab, (batch, 1), device=device)
 
     def step():
-        b = PagedBatch.of(table, past, 1, page_size)
+        b = paged.PagedBatch.of(table, past, 1, page_size)
         logits = model(cur, pos=b.pos, caches=b.over(caches))
         cur.copy_(logits.argmax(-1))
         past.add_(1)

@@ -27,6 +27,7 @@ import torch.nn.functional as F
 
 from ..models.llama import (CONFIGS, Llama, LlamaConfig, RMSNorm,
                             apply_rope, is_paged, paged_caches)
+from ..ops import paged
 
 
 def _world():
@@ -86,7 +87,6 @@ class TPAttention(nn.Module):
                 mask=None):
         B, T, _ = x.shape
         if is_paged(cache, mask):
-            from ..ops import paged
             o = paged.attend(*(w(x).flatten(0, 1) for w in (self.wq, self.wk,
                                                             self.wv)),
                              cos, sin, *cache, self.heads)
