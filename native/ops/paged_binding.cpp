@@ -373,7 +373,12 @@ struct Plan {
 };
 
 // Which kernel attends, and how it shares the keys. What a batch holds lies
-// on the device; this goes by its mean, and is right for any batch. Up to 16
+// on the device; this goes by the mean number of rows a sequence and by the keys
+// that the table could hold, and is right for any batch. It costs time where
+// that is far from what the batch holds: 8 steps on 560 keys take 9.5 us in a
+// table for 560 and 13.9 in one for 8192, 64 such steps 28.2 and 42.5 (32 / 8
+// heads, D = 128, 16 bits); 200 steps on 500 to 4000 keys and 512 tokens over
+// 4000 take 466 us in one call and 407 in two. Up to 16
 // rows (new tokens * G) a sequence are work for the kernel for few rows, whose
 // `workers` share it out among themselves; 0 workers: the kernel for many
 // rows, with the keys of each tile of 128 rows in `splits` parts.

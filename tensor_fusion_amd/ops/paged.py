@@ -152,7 +152,8 @@ class PagedBatch:
         """`new` tokens (a number, or one for each sequence) behind the
         first `past` (integers [B]) of the sequences of a block table. With
         a number everything is worked out on the device, so that a step that
-        is captured goes on from wherever `past` stands at the replay."""
+        is captured goes on from wherever `past` stands at the replay. A list
+        is worked out on the host, and its copies wait for the stream."""
 
         if page_size < 1:
             raise ValueError(f"no page_size of {page_size}")
@@ -189,7 +190,8 @@ class PagedBatch:
                    page_size)
 
     def check(self, cache: PagedKVCache) -> None:
-        if self.page_size is not None and self.page_size != cache.page_size:
+        size = self.page_size
+        if size is not None and size != cache._tensors[0].shape[2]:
             raise ValueError(f"a batch for pages of {self.page_size} tokens, "
                              f"and a cache with pages of {cache.page_size}")
 
@@ -274,7 +276,14 @@ def paged_attention(q, cache: PagedKVCache, q_starts, kv_lens, block_table,
     number is outside of the pool is NaN, and so are all rows of a sequence
     whose length is negative or more than its table holds. A quantised
     cache's values enter as q's type; for fp16 a value past 65504, which only
-    rows of bf16 can have left there, is an infinity."""
+    rows of bf16 can have left there, is an infinity. The weights of the keys
+    are rounded to q's type for their product with the values, as the result
+    is; sums are 32 bits.
+
+    The host sees sizes only: which kernel runs goes by the mean number of new
+    tokens, and how it shares the keys by the table's columns. Many steps next
+    to a long chunk are sooner done in two calls, and short sequences in a
+    table that is not much wider than they are."""
 
     return (_EXT or _ext()).attention(cache._pools, q, q_starts, kv_lens,
                                       block_table, scale, causal, out)
