@@ -415,11 +415,11 @@ int tf_accel_set_compute_partition(int device, const char* mode) {
     s.mock_compute_mode[device] = mode;
     return TF_ACCEL_OK;
   }
-  if (!s.api.set_compute_partition) return TF_ACCEL_NOT_SUPPORTED;
   char now[32] = "";  // the mode it is in needs neither change nor privilege
   if (tf_accel_get_compute_partition(device, now, sizeof now) == TF_ACCEL_OK &&
       compute_mode_enum(now) == e)
     return TF_ACCEL_OK;
+  if (!s.api.set_compute_partition) return TF_ACCEL_NOT_SUPPORTED;
   return s.api.set_compute_partition(s.procs[device], (uint32_t)e) == 0
              ? TF_ACCEL_OK
              : TF_ACCEL_ERR;
@@ -450,11 +450,11 @@ int tf_accel_set_memory_partition(int device, const char* mode) {
     s.mock_memory_mode[device] = mode;
     return TF_ACCEL_OK;
   }
-  if (!s.api.set_memory_partition) return TF_ACCEL_NOT_SUPPORTED;
   char now[32] = "";  // the mode it is in needs neither change nor privilege
   if (tf_accel_get_memory_partition(device, now, sizeof now) == TF_ACCEL_OK &&
       memory_mode_enum(now) == e)
     return TF_ACCEL_OK;
+  if (!s.api.set_memory_partition) return TF_ACCEL_NOT_SUPPORTED;
   return s.api.set_memory_partition(s.procs[device], (uint32_t)e) == 0
              ? TF_ACCEL_OK
              : TF_ACCEL_ERR;

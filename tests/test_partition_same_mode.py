@@ -1,6 +1,6 @@
 """Setting the partition mode that a device is in already: nothing to do, and
-no privilege to ask for. Against a stand-in for the management library whose
-setters fail, as they do for an unprivileged process."""
+no privilege to ask for. Against a stand-in for the management library that
+has no setters."""
 import os
 import subprocess
 import sys
@@ -44,8 +44,6 @@ int amdsmi_get_gpu_memory_partition(void*, char* m, uint32_t n) {
   snprintf(m, n, "NPS1");
   return 0;
 }
-int amdsmi_set_gpu_compute_partition(void*, uint32_t) { return 10; }
-int amdsmi_set_gpu_memory_partition(void*, uint32_t) { return 10; }
 }
 """
 
@@ -56,9 +54,10 @@ assert a.devices()[0].uuid == "GPU-stand-in", a.devices()
 assert (a.compute_partition(0), a.memory_partition(0)) == ("SPX", "NPS1")
 assert a.set_compute_partition(0, "SPX") and a.set_compute_partition(0, "spx")
 assert a.set_memory_partition(0, "NPS1")
-for change in (lambda: a.set_compute_partition(0, "CPX"),
-               lambda: a.set_memory_partition(0, "NPS4"),
-               lambda: a.set_compute_partition(0, "BOGUS"),
+assert not a.set_compute_partition(0, "CPX")
+assert not a.set_memory_partition(0, "NPS4")
+for change in (lambda: a.set_compute_partition(0, "BOGUS"),
+               lambda: a.set_memory_partition(0, "NPS3"),
                lambda: a.set_compute_partition(1, "SPX")):
     try:
         change()
