@@ -1664,8 +1664,9 @@ int tf_paged_attention(
          (float*)parts, nullptr, q_row, q_head, table_row, cols, T, B, Hq, Hk,
          Hq / Hk, pages, page_log2,
          (uint32_t)(((1ULL << 32) + Hq / Hk - 1) / (Hq / Hk)),
-         // 0 times a masked score would be NaN; this leaves every p 1 too
-         scale == 0.0f ? 1e-38f : scale * 1.4426950408889634f, causal, 1, 0, 1, 0};
+         // 0 times a masked score would be NaN; this leaves every p 1 too, to
+         // 2^-21 for the largest scores (1e-38 did not: they reach 3e38)
+         scale == 0.0f ? 0x1p-149f : scale * 1.4426950408889634f, causal, 1, 0, 1, 0};
   // a line of less than 2^30 units, as bounded by what the host knows
   const double items = ((double)T * (Hq / Hk) / 16 + B) * Hk;
   while (items * (OWN + ((double)cols * (1 << page_log2) /

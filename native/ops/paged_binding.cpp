@@ -643,8 +643,9 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[5] != Py_None) {
       scale = PyFloat_AsDouble(a[5]);
       if (PyErr_Occurred()) return nullptr;
-      if (!std::isfinite((float)scale))
-        refuse("scale is a finite number: got ", scale);
+      // the kernels' exponentials are of base 2
+      if (!std::isfinite((float)scale * 1.4426950408889634f))
+        refuse("scale is a finite number, and times log2(e): got ", scale);
     }
     const int causal = PyObject_IsTrue(a[6]);
     if (causal < 0) return nullptr;

@@ -150,3 +150,25 @@ def test_under_inference_mode():
         slots = torch.arange(3, device="cuda")
         paged.kv_write(b.cache, k, k, slots)
         assert torch.equal(paged.kv_read(b.cache, slots)[0], k)
+
+
+# ---- scales -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seqs", [[(1, 90), (3, 40)], [(2, 5000)],
+                                  [(130, 200)]],
+                         ids=["few", "shared", "many"])
+@KEPT
+def test_no_scale_of_large_scores(seqs, quantized):
+    """Scores of up to 2^128 and a scale of 0, or of less than 32 bits hold:
+    every key has the same weight. (2^128 times the 2^-149 that stands for it
+    is 2^-21, far below half a step of p.)"""
+
+    b = Batch(seqs, 8, 2, 64, 16, BF16, quantized, seed=2)
+    if quantized:
+        b.cache.k_scale.add_(58)
+    else:
+        b.cache.k.mul_(2.0 ** 58)
+    b.q = b.q * 2.0 ** 60  # products of up to 64 * 4 * 4 * 2^118 < 2^128
+    for scale in (0.0, 1e-60, -0.0):
+        check(b.run(scale=scale), *b.want(scale=0.0))

@@ -287,3 +287,14 @@ def test_a_batch_of_another_page_size():
     for page in (0, -16):
         with pytest.raises(ValueError, match="page_size"):
             batch_of(page)
+
+
+def test_scales_that_32_bits_do_not_hold():
+    """Exponentials are of base 2: the scale times log2(e) has to be finite."""
+
+    for scale in (2.4e38, -3e38, 1e39, float("inf")):
+        with pytest.raises(ValueError, match="finite"):
+            attend(cache(), scale=scale)
+    for scale in (2.3e38, -2.3e38, 0.0, 1e-45, 1e-60):
+        with pytest.raises(ValueError, match="run on a GPU"):
+            attend(cache(), scale=scale)
